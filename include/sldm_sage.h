@@ -37,7 +37,7 @@
 extern "C" {
 #endif
 
-#define SLDM_ABI_VERSION 9   /* 9: + sldm_set_dropout_seed_source; 8: + sldm_gemm_nt_rowscale_blocked(_ok) */
+#define SLDM_ABI_VERSION 10  /* 10: + layer norm, rotary positions, decay attention; 9: + sldm_set_dropout_seed_source; 8: + sldm_gemm_nt_rowscale_blocked(_ok) */
 
 enum sldm_dtype { SLDM_F32 = 0, SLDM_BF16 = 1 };
 enum sldm_status { SLDM_OK = 0, SLDM_ERR_ARG = 1, SLDM_ERR_HIP = 2 };
@@ -399,6 +399,84 @@ int sldm_gru_bwd(const float* x, int64_t ldx_n, int64_t ldx_t, int64_t N, int64_
                  int64_t lddx_n, int64_t lddx_t, float* dh0, float* dw_ih, float* dw_hh,
                  float* db_ih, float* db_hh, void* workspace, size_t workspace_bytes,
                  void* stream);
+
+/* ------------------------------------------------------ sequence encoder ---
+ * The operators of a trajectory encoder that mixes a vehicle's frames without
+ * a GRU (sldm_sage/sequence.py): no counterpart in the reference, whose
+ * encoder is the GRU above (grusage.py:66-71).
+ *
+ * Layer norm over rows of `width` contiguous elements (x: row stride ldx, dy:
+ * lddy; y and dx contiguous):
+ *   y = (x - mean) rstd weight + bias,   rstd = 1 / sqrt(var_biased + eps)
+ * weight / bias (fp32) nullable; mean / rstd (fp32 [rows], both or neither)
+ * are what the backward needs. */
+int sldm_layer_norm_fwd(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t width,
+                        const float* weight, const float* bias, float eps, void* y, float* mean,
+                        float* rstd, void* stream);
+/* dx, dweight, dbias (each nullable) of sldm_layer_norm_fwd; the columns' sums
+ * are taken in a fixed order (deterministic) and are zeros for rows == 0. */
+size_t sldm_layer_norm_bwd_workspace_bytes(int dtype, int64_t rows, int64_t width);
+int sldm_layer_norm_bwd(int dtype, const void* x, int64_t ldx, const void* dy, int64_t lddy,
+                        int64_t rows, int64_t width, const float* weight, const float* mean,
+                        const float* rstd, void* dx, float* dweight, float* dbias,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rotary positions over several axes: q [B, T, heads_q, dim] and k [B, T,
+ * heads_k, dim] (heads_k == 0: no k) are turned pair by pair, pair p of axis a
+ * by positions[b, t, a] * inv_freq[p] (`inverse`: by minus that, which is the
+ * gradient).  Axis 0 owns the first sections[0] pairs, axis 1 the next
+ * sections[1], ...; pair p is (p, p + P) with P the sum of the sections, or
+ * (2p, 2p + 1) if interleaved; columns from 2P on are copied.  ld_*: HOST
+ * arrays of three element strides (batch, token, head; positions: batch,
+ * token, axis); columns are contiguous.  out_q / out_k: contiguous, not the
+ * inputs.  sections: HOST array.  inv_freq: fp64 [P].  Angles are computed in
+ * fp64.  1 <= num_axes <= 8, dim <= 1024. */
+enum sldm_pos_type { SLDM_POS_I32 = 0, SLDM_POS_I64 = 1, SLDM_POS_F32 = 2, SLDM_POS_F64 = 3 };
+int sldm_rotary_axes(int dtype, const void* q, const int64_t* ld_q, int64_t heads_q, const void* k,
+                     const int64_t* ld_k, int64_t heads_k, int64_t B, int64_t T, int64_t dim,
+                     const void* positions, int pos_type, const int64_t* ld_pos,
+                     const double* inv_freq, const int64_t* sections, int64_t num_axes,
+                     int interleaved, int inverse, void* out_q, void* out_k, void* stream);
+
+/* Linear attention with a decay for each head:
+ *   S_t = g S_{t-1} + k_t v_t^T,  o_t = scale q_t S_t,   g = exp(log_decay[h])
+ * q [B, T, H, dk], k [B, T, Hk, dk], v [B, T, Hk, dv] (head h reads key head
+ * h / (H / Hk)); ld_*: HOST arrays of three element strides (batch, token,
+ * head), columns contiguous.  state (nullable: zeros) and state_out (nullable)
+ * [B, H, dk, dv] fp32 contiguous: the state before the first token and behind
+ * the last.  lengths (device [B], int32 or int64, nullable: T): tokens from
+ * lengths[b] on (clamped to [0, T]) are padding: not read into the state, their
+ * outputs are zeros.  out [B, T, H, dv] contiguous.  1 <= dk, dv <= 128.
+ * log_decay [H] fp32, <= 0 (-inf: nothing is kept).
+ * workspace: sldm_decay_attention_workspace_bytes(.., backward). */
+size_t sldm_decay_attention_workspace_bytes(int dtype, int64_t B, int64_t T, int64_t H, int64_t Hk,
+                                            int64_t dk, int64_t dv, int backward);
+int sldm_decay_attention_fwd(int dtype, const void* q, const int64_t* ld_q, const void* k,
+                             const int64_t* ld_k, const void* v, const int64_t* ld_v, int64_t B,
+                             int64_t T, int64_t H, int64_t Hk, int64_t dk, int64_t dv,
+                             const float* log_decay, float scale, const float* state,
+                             const void* lengths, int lengths_int64, void* out, float* state_out,
+                             void* workspace, size_t workspace_bytes, void* stream);
+/* Gradients of sldm_decay_attention_fwd with respect to q, k, v and state
+ * (contiguous, each nullable; padding tokens get zeros).  dout has `out`'s
+ * shape with strides ld_do; dstate_out (nullable: zeros) is state_out's
+ * gradient.  Shared key heads: the group's parts are added in fp32, in order. */
+int sldm_decay_attention_bwd(int dtype, const void* q, const int64_t* ld_q, const void* k,
+                             const int64_t* ld_k, const void* v, const int64_t* ld_v,
+                             const void* dout, const int64_t* ld_do, int64_t B, int64_t T,
+                             int64_t H, int64_t Hk, int64_t dk, int64_t dv,
+                             const float* log_decay, float scale, const float* state,
+                             const float* dstate_out, const void* lengths, int lengths_int64,
+                             void* dq, void* dk_out, void* dv_out, float* dstate, void* workspace,
+                             size_t workspace_bytes, void* stream);
+/* One token for each sequence, the state [B, H, dk, dv] moved on in place:
+ * q [B, H, dk], k [B, Hk, dk], v [B, Hk, dv] with ld_* = HOST {batch, head}
+ * strides, out [B, H, dv] contiguous. */
+int sldm_decay_attention_step(int dtype, const void* q, const int64_t* ld_q, const void* k,
+                              const int64_t* ld_k, const void* v, const int64_t* ld_v, int64_t B,
+                              int64_t H, int64_t Hk, int64_t dk, int64_t dv,
+                              const float* log_decay, float scale, float* state, void* out,
+                              void* stream);
 
 #ifdef __cplusplus
 }

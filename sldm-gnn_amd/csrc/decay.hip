@@ -1,0 +1,393 @@
+// Host side of the decay attention operators (kernel: decay.hpp), the scan
+// that joins the segments of a long axis, the sum over shared heads, and the
+// single-token step.
+#include <algorithm>
+
+#include "decay.hpp"
+
+namespace sldm_decay {
+namespace {
+
+constexpr int kMaxDim = 128;
+constexpr int64_t kMaxThreads = (int64_t)1 << 32;   // work-items of one launch, exclusive
+
+int chunk_of(int dtype) { return dtype == SLDM_F32 ? 32 : 64; }
+
+// Segments of the time axis.  One workgroup walks a sequence alone unless that
+// leaves the chip short of waves (256 CUs x 4 SIMDs x 2); then the axis is cut
+// into pieces of at least 4 chunks, at the price of a pass over k and v for
+// the pieces' states.
+struct Plan {
+  int64_t seg_len;
+  int nseg;
+};
+Plan plan(int dtype, int64_t B, int64_t H, int64_t T, int64_t dk, int64_t dv, int roles) {
+  const int64_t C = chunk_of(dtype);
+  const int64_t waves = B * H * roles * std::max(tiles_of((int)dk), tiles_of((int)dv));
+  const int64_t chunks = (T + C - 1) / C;
+  int64_t want = waves > 0 ? 2048 / waves : 1;
+  want = std::min(want, chunks / 4);
+  if (want <= 1) return {std::max<int64_t>(T, 1), 1};
+  const int64_t per = (chunks + want - 1) / want;
+  return {per * C, (int)((chunks + per - 1) / per)};
+}
+
+// loc[bh][s]: the states that segments add, each from zero -> the states
+// before each segment, and the state behind the last one.
+__global__ __launch_bounds__(256) void scan_kernel(float* loc, const float* s0, float* s1, Args a,
+                                                   int64_t elems) {
+  const int64_t bh = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (bh >= a.B * a.H || e >= elems) return;
+  const int64_t len = seq_len(a, bh / a.H);
+  const float ld2 = a.log_decay[bh % a.H] * 1.44269504088896340736f;
+  float run = s0 ? s0[bh * elems + e] : 0.f;
+  float* p = loc + bh * a.nseg * elems + e;
+  const float g = exp2f(ld2 * (float)a.seg_len);
+  int s = 0;
+  for (; s < a.nseg && (int64_t)(s + 1) * a.seg_len <= len; ++s) {
+    const float add = p[s * elems];
+    p[s * elems] = run;
+    run = run * g + add;
+  }
+  if (s < a.nseg) {
+    const int64_t n = len - (int64_t)s * a.seg_len;
+    const float add = p[s * elems];
+    p[s * elems] = run;
+    run = run * powg(ld2, (int)n) + add;
+    for (++s; s < a.nseg; ++s) p[s * elems] = run;
+  }
+  if (s1) s1[bh * elems + e] = run;
+}
+
+// out[b, t, hk, :] = sum over the group's heads of part[b, t, hk * group + g, :]
+template <typename T>
+__global__ __launch_bounds__(256) void sum_heads_kernel(const float* part, T* out, int64_t n, int group,
+                                                        int d) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t head = i / d;
+    const float* p = part + head * group * d + i % d;
+    float s = p[0];
+    for (int g = 1; g < group; ++g) s += p[(int64_t)g * d];
+    if constexpr (sizeof(T) == 4) out[i] = s;
+    else out[i] = sldm::f32_to_bf16(s);
+  }
+}
+
+// One token: S <- g S + k v^T and o = scale q S, the state read and written
+// once (its 8 Dk Dv bytes are all that counts).  A workgroup owns one (batch,
+// head); lanes hold V neighbouring value columns, the row groups' partial sums
+// of o meet in LDS.
+struct StepArgs {
+  const void *q, *k, *v;
+  int64_t q_sb, q_sh, k_sb, k_sh, v_sb, v_sh;
+  void* o;
+  float* state;
+  const float* log_decay;
+  int64_t H;
+  int group, dk, dv, cols;   // cols: lanes across the value columns (a power of two)
+  float scale;
+};
+template <typename T> __device__ __forceinline__ float as_f32(T v);
+template <> __device__ __forceinline__ float as_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ float as_f32<uint16_t>(uint16_t v) { return sldm::bf16_to_f32(v); }
+
+template <typename T, int V, int NTH>
+__global__ __launch_bounds__(NTH) void step_kernel(StepArgs a) {
+  __shared__ float qs[kMaxDim], ks[kMaxDim], red[NTH * V];
+  const int64_t bh = blockIdx.x, b = bh / a.H, hd = bh % a.H, hk = hd / a.group;
+  const T* q = reinterpret_cast<const T*>(a.q) + b * a.q_sb + hd * a.q_sh;
+  const T* k = reinterpret_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh;
+  const T* v = reinterpret_cast<const T*>(a.v) + b * a.v_sb + hk * a.v_sh;
+  const int tid = threadIdx.x, col = tid & (a.cols - 1), grp = tid / a.cols, groups = NTH / a.cols;
+  for (int i = tid; i < a.dk; i += NTH) {
+    qs[i] = as_f32(q[i]) * a.scale;
+    ks[i] = as_f32(k[i]);
+  }
+  const int c0 = col * V;
+  const bool on = c0 < a.dv;
+  float vv[V], acc[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    vv[e] = on ? as_f32(v[c0 + e]) : 0.f;
+    acc[e] = 0.f;
+  }
+  const float g = expf(a.log_decay[hd]);
+  __syncthreads();
+  float* s = a.state + bh * a.dk * a.dv + c0;
+  if (on) {
+#pragma unroll 4
+    for (int r = grp; r < a.dk; r += groups) {
+      float w[V];
+      sldm::Vec<float, V>::load(s + (int64_t)r * a.dv, w);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        w[e] = w[e] * g + ks[r] * vv[e];
+        acc[e] += qs[r] * w[e];
+      }
+      sldm::Vec<float, V>::store(s + (int64_t)r * a.dv, w);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < V; ++e) red[grp * a.cols * V + c0 + e] = acc[e];
+  __syncthreads();
+  T* o = reinterpret_cast<T*>(a.o) + bh * a.dv;
+  for (int c = tid; c < a.dv; c += NTH) {
+    float sum = 0.f;
+    for (int r = 0; r < groups; ++r) sum += red[r * a.cols * V + c];
+    if constexpr (sizeof(T) == 4) o[c] = sum;
+    else o[c] = sldm::f32_to_bf16(sum);
+  }
+}
+
+Operand operand(const void* p, const int64_t* ld, int hdiv, int esz) {
+  Operand t{p, ld[0], ld[1], ld[2], hdiv, 1};
+  for (int i = 0; i < 3; ++i) t.vec &= (ld[i] * esz) % 16 == 0;
+  t.vec &= reinterpret_cast<uintptr_t>(p) % 16 == 0;
+  return t;
+}
+
+void set_out(Role& r, void* o, int64_t T, int64_t H, int64_t d, bool f32, int esz) {
+  r.o = o;
+  r.o_sb = T * H * d;
+  r.o_st = H * d;
+  r.o_sh = d;
+  r.o_f32 = f32;
+  r.o_vec = (d * (f32 ? 4 : esz)) % 16 == 0 && reinterpret_cast<uintptr_t>(o) % 16 == 0;
+}
+
+void launch_roles(int dtype, Args& a, const Role* const* roles, int n, bool out, hipStream_t st) {
+  // roles of the same tile classes share a launch
+  bool done[3] = {false, false, false};
+  for (int i = 0; i < n; ++i) {
+    if (done[i]) continue;
+    int m = 0;
+    for (int j = i; j < n; ++j)
+      if (!done[j] && tiles_of(roles[j]->kd) == tiles_of(roles[i]->kd) &&
+          tiles_of(roles[j]->vd) == tiles_of(roles[i]->vd)) {
+        a.role[m++] = *roles[j];
+        done[j] = true;
+      }
+    if (dtype == SLDM_F32) run_f32(a, m, out, st);
+    else run_bf16(a, m, out, st);
+  }
+}
+
+int scan(float* loc, const float* s0, float* s1, const Args& a, int64_t elems, hipStream_t st) {
+  const int64_t bh = a.B * a.H;
+  const int64_t y = std::min<int64_t>(bh, 32768);
+  scan_kernel<<<dim3((unsigned)((elems + 255) / 256), (unsigned)y, (unsigned)((bh + y - 1) / y)), 256, 0, st>>>(
+      loc, s0, s1, a, elems);
+  SLDM_LAUNCH_CHECK("decay scan_kernel");
+  return SLDM_OK;
+}
+
+int check_shape(int dtype, int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t dk, int64_t dv) {
+  SLDM_REQUIRE(dtype == SLDM_F32 || dtype == SLDM_BF16, "decay attention: dtype must be fp32 or bf16");
+  SLDM_REQUIRE(B >= 0 && T >= 0 && T < ((int64_t)1 << 31), "decay attention: B and T must be >= 0, T < 2^31");
+  SLDM_REQUIRE(H >= 1 && Hk >= 1 && H % Hk == 0, "decay attention: %lld heads over %lld key heads",
+               (long long)H, (long long)Hk);
+  SLDM_REQUIRE(dk >= 1 && dk <= kMaxDim && dv >= 1 && dv <= kMaxDim,
+               "decay attention: head sizes must be in [1, %d], got %lld and %lld", kMaxDim, (long long)dk,
+               (long long)dv);
+  SLDM_REQUIRE(B * H < kMaxThreads / 256, "decay attention: too many (batch, head) pairs: %lld",
+               (long long)(B * H));
+  return SLDM_OK;
+}
+
+}  // namespace
+}  // namespace sldm_decay
+
+using namespace sldm_decay;
+
+extern "C" size_t sldm_decay_attention_workspace_bytes(int dtype, int64_t B, int64_t T, int64_t H, int64_t Hk,
+                                                       int64_t dk, int64_t dv, int backward) {
+  if (check_shape(dtype, B, T, H, Hk, dk, dv) != SLDM_OK) return 0;
+  const Plan p = plan(dtype, B, H, T, dk, dv, backward ? 3 : 1);
+  size_t n = p.nseg > 1 ? (size_t)(B * H) * p.nseg * dk * dv * (backward ? 2 : 1) : 0;
+  if (backward && H != Hk) n += (size_t)(B * T * H) * (dk + dv);
+  return n * 4 + 256;
+}
+
+extern "C" int sldm_decay_attention_fwd(int dtype, const void* q, const int64_t* ld_q, const void* k,
+                                        const int64_t* ld_k, const void* v, const int64_t* ld_v, int64_t B,
+                                        int64_t T, int64_t H, int64_t Hk, int64_t dk, int64_t dv,
+                                        const float* log_decay, float scale, const float* state,
+                                        const void* lengths, int lengths_int64, void* out, float* state_out,
+                                        void* workspace, size_t workspace_bytes, void* stream) {
+  if (const int rc = check_shape(dtype, B, T, H, Hk, dk, dv)) return rc;
+  if (B == 0) return SLDM_OK;
+  SLDM_REQUIRE(ld_q && ld_k && ld_v && log_decay, "sldm_decay_attention_fwd: null argument");
+  SLDM_REQUIRE(T == 0 || (q && k && v && out), "sldm_decay_attention_fwd: null argument");
+  SLDM_REQUIRE(workspace_bytes >= sldm_decay_attention_workspace_bytes(dtype, B, T, H, Hk, dk, dv, 0) && workspace,
+               "sldm_decay_attention_fwd: workspace too small");
+  const int esz = dtype == SLDM_F32 ? 4 : 2, group = (int)(H / Hk);
+  const Plan p = plan(dtype, B, H, T, dk, dv, 1);
+  const int64_t elems = dk * dv;
+  hipStream_t st = sldm::as_stream(stream);
+  Args a{};
+  a.B = B; a.H = H; a.T = T;
+  a.seg_len = p.seg_len; a.nseg = p.nseg; a.groups = (int)(B * H * p.nseg);
+  a.log_decay = log_decay; a.lengths = lengths; a.lengths64 = lengths_int64;
+  Role r{};
+  r.q = operand(q, ld_q, 1, esz);
+  r.k = operand(k, ld_k, group, esz);
+  r.v = operand(v, ld_v, group, esz);
+  set_out(r, out, T, H, dv, false, esz);
+  r.kd = (int)dk; r.vd = (int)dv;
+  r.s_k = dv; r.s_v = 1;
+  r.read_scale = r.p_scale = scale;
+  r.upd_scale = 1.f;
+  const Role* one[1] = {&r};
+  if (p.nseg == 1) {
+    r.s0 = state; r.s0_bh = elems;
+    r.s1 = state_out; r.s1_bh = elems;
+    launch_roles(dtype, a, one, 1, true, st);
+    SLDM_LAUNCH_CHECK("decay_kernel");
+    return SLDM_OK;
+  }
+  float* loc = reinterpret_cast<float*>(workspace);
+  r.s1 = loc; r.s1_bh = p.nseg * elems; r.s1_seg = elems;
+  launch_roles(dtype, a, one, 1, false, st);
+  SLDM_LAUNCH_CHECK("decay_kernel (states)");
+  if (const int rc = scan(loc, state, state_out, a, elems, st)) return rc;
+  r.s1 = nullptr;
+  r.s0 = loc; r.s0_bh = p.nseg * elems; r.s0_seg = elems;
+  launch_roles(dtype, a, one, 1, true, st);
+  SLDM_LAUNCH_CHECK("decay_kernel");
+  return SLDM_OK;
+}
+
+extern "C" int sldm_decay_attention_bwd(int dtype, const void* q, const int64_t* ld_q, const void* k,
+                                        const int64_t* ld_k, const void* v, const int64_t* ld_v, const void* dout,
+                                        const int64_t* ld_do, int64_t B, int64_t T, int64_t H, int64_t Hk,
+                                        int64_t dk, int64_t dv, const float* log_decay, float scale,
+                                        const float* state, const float* dstate_out, const void* lengths,
+                                        int lengths_int64, void* dq, void* dk_out, void* dv_out, float* dstate,
+                                        void* workspace, size_t workspace_bytes, void* stream) {
+  if (const int rc = check_shape(dtype, B, T, H, Hk, dk, dv)) return rc;
+  if (B == 0) return SLDM_OK;
+  SLDM_REQUIRE(ld_q && ld_k && ld_v && ld_do && log_decay, "sldm_decay_attention_bwd: null argument");
+  SLDM_REQUIRE(T == 0 || (q && k && v && dout), "sldm_decay_attention_bwd: null argument");
+  SLDM_REQUIRE(workspace_bytes >= sldm_decay_attention_workspace_bytes(dtype, B, T, H, Hk, dk, dv, 1) && workspace,
+               "sldm_decay_attention_bwd: workspace too small");
+  const int esz = dtype == SLDM_F32 ? 4 : 2, group = (int)(H / Hk);
+  const Plan p = plan(dtype, B, H, T, dk, dv, 3);
+  const int64_t elems = dk * dv;
+  hipStream_t st = sldm::as_stream(stream);
+  Args a{};
+  a.B = B; a.H = H; a.T = T;
+  a.seg_len = p.seg_len; a.nseg = p.nseg; a.groups = (int)(B * H * p.nseg);
+  a.log_decay = log_decay; a.lengths = lengths; a.lengths64 = lengths_int64;
+
+  float* ws = reinterpret_cast<float*>(workspace);
+  float *locS = nullptr, *locR = nullptr, *part_k = nullptr, *part_v = nullptr;
+  if (p.nseg > 1) {
+    locS = ws; ws += B * H * p.nseg * elems;
+    locR = ws; ws += B * H * p.nseg * elems;
+  }
+  if (group > 1) {
+    part_k = ws; ws += B * T * H * dk;
+    part_v = ws;
+  }
+  const Operand oq = operand(q, ld_q, 1, esz), ok = operand(k, ld_k, group, esz),
+                ov = operand(v, ld_v, group, esz), od = operand(dout, ld_do, 1, esz);
+
+  Role rq{}, rk{}, rv{};
+  rq.q = od; rq.k = ov; rq.v = ok;               // dq_t = scale S_t do_t
+  rq.kd = (int)dv; rq.vd = (int)dk;
+  rq.s_k = 1; rq.s_v = dv;
+  rq.read_scale = rq.p_scale = scale; rq.upd_scale = 1.f;
+  set_out(rq, dq, T, H, dk, false, esz);
+  rv.q = ok; rv.k = oq; rv.v = od;               // dv_t = k_t G_t
+  rv.kd = (int)dk; rv.vd = (int)dv;
+  rv.s_k = dv; rv.s_v = 1;
+  rv.read_scale = 1.f; rv.p_scale = rv.upd_scale = scale;
+  rv.delta = rv.reverse = 1;
+  set_out(rv, group > 1 ? (void*)part_v : dv_out, T, H, dv, group > 1, esz);
+  rk.q = ov; rk.k = od; rk.v = oq;               // dk_t = G_t v_t
+  rk.kd = (int)dv; rk.vd = (int)dk;
+  rk.s_k = 1; rk.s_v = dv;
+  rk.read_scale = 1.f; rk.p_scale = rk.upd_scale = scale;
+  rk.delta = rk.reverse = 1;
+  set_out(rk, group > 1 ? (void*)part_k : dk_out, T, H, dk, group > 1, esz);
+
+  if (p.nseg > 1) {
+    Role s{}, g = rv;                            // states that each segment adds
+    s.k = ok; s.v = ov;
+    s.kd = (int)dk; s.vd = (int)dv;
+    s.s_k = dv; s.s_v = 1;
+    s.upd_scale = 1.f;
+    s.s1 = locS; g.s1 = locR;
+    s.s1_bh = g.s1_bh = p.nseg * elems;
+    s.s1_seg = g.s1_seg = elems;
+    const Role* two[2];
+    int n = 0;
+    if (dq) two[n++] = &s;
+    if (dk_out || dv_out || dstate) two[n++] = &g;
+    launch_roles(dtype, a, two, n, false, st);
+    SLDM_LAUNCH_CHECK("decay_kernel (states)");
+    if (dq)
+      if (const int rc = scan(locS, state, nullptr, a, elems, st)) return rc;
+    if (dk_out || dv_out || dstate)
+      if (const int rc = scan(locR, dstate_out, dstate, a, elems, st)) return rc;
+    rq.s0 = locS; rk.s0 = rv.s0 = locR;
+    rq.s0_bh = rk.s0_bh = rv.s0_bh = p.nseg * elems;
+    rq.s0_seg = rk.s0_seg = rv.s0_seg = elems;
+  } else {
+    rq.s0 = state; rk.s0 = rv.s0 = dstate_out;
+    rq.s0_bh = rk.s0_bh = rv.s0_bh = elems;
+    rv.s1 = dstate; rv.s1_bh = elems;
+    if (dstate && !dv_out) {                     // the state's gradient alone
+      const Role* one[1] = {&rv};
+      launch_roles(dtype, a, one, 1, false, st);
+      SLDM_LAUNCH_CHECK("decay_kernel (states)");
+    }
+  }
+  const Role* roles[3];
+  int n = 0;
+  if (dq) roles[n++] = &rq;
+  if (dk_out) roles[n++] = &rk;
+  if (dv_out) roles[n++] = &rv;
+  launch_roles(dtype, a, roles, n, true, st);
+  SLDM_LAUNCH_CHECK("decay_kernel");
+  if (group > 1 && T > 0) {
+    for (int i = 0; i < 2; ++i) {
+      void* out = i ? dv_out : dk_out;
+      if (!out) continue;
+      const int d = (int)(i ? dv : dk);
+      const int64_t cnt = B * T * Hk * d;
+      const unsigned grid = (unsigned)std::min<int64_t>((cnt + 255) / 256, 1 << 16);
+      if (dtype == SLDM_F32)
+        sum_heads_kernel<float><<<grid, 256, 0, st>>>(i ? part_v : part_k, (float*)out, cnt, group, d);
+      else
+        sum_heads_kernel<uint16_t><<<grid, 256, 0, st>>>(i ? part_v : part_k, (uint16_t*)out, cnt, group, d);
+      SLDM_LAUNCH_CHECK("decay sum_heads_kernel");
+    }
+  }
+  return SLDM_OK;
+}
+
+extern "C" int sldm_decay_attention_step(int dtype, const void* q, const int64_t* ld_q, const void* k,
+                                         const int64_t* ld_k, const void* v, const int64_t* ld_v, int64_t B,
+                                         int64_t H, int64_t Hk, int64_t dk, int64_t dv, const float* log_decay,
+                                         float scale, float* state, void* out, void* stream) {
+  if (const int rc = check_shape(dtype, B, 1, H, Hk, dk, dv)) return rc;
+  if (B == 0) return SLDM_OK;
+  SLDM_REQUIRE(q && k && v && ld_q && ld_k && ld_v && log_decay && state && out,
+               "sldm_decay_attention_step: null argument");
+  StepArgs a{q, k, v, ld_q[0], ld_q[1], ld_k[0], ld_k[1], ld_v[0], ld_v[1], out, state, log_decay, H,
+             (int)(H / Hk), (int)dk, (int)dv, 1, scale};
+  const bool vec = dv % 4 == 0 && reinterpret_cast<uintptr_t>(state) % 16 == 0;
+  while (a.cols * (vec ? 4 : 1) < dv) a.cols <<= 1;
+  const bool small = dk * dv <= 1024;   // a wave holds such a state; four waves a larger one
+  const unsigned grid = (unsigned)(B * H);
+  hipStream_t st = sldm::as_stream(stream);
+#define SLDM_STEP(T, V) \
+  (small ? step_kernel<T, V, 128><<<grid, 128, 0, st>>>(a) : step_kernel<T, V, 256><<<grid, 256, 0, st>>>(a))
+  if (dtype == SLDM_F32) vec ? SLDM_STEP(float, 4) : SLDM_STEP(float, 1);
+  else vec ? SLDM_STEP(uint16_t, 4) : SLDM_STEP(uint16_t, 1);
+#undef SLDM_STEP
+  SLDM_LAUNCH_CHECK("step_kernel");
+  return SLDM_OK;
+}

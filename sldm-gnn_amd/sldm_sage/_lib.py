@@ -15,7 +15,7 @@ import torch  # noqa: F401  (must be imported before the HIP library)
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SLDM_SAGE_LIB", os.path.join(_HERE, "libsldm_sage.so"))
 
-ABI_VERSION = 9
+ABI_VERSION = 10
 F32, BF16 = 0, 1
 
 _c_i64 = ctypes.c_int64
@@ -107,6 +107,30 @@ _SIGNATURES = {
                                     _vp, _vp, _vp, _c_i64, _c_i64, _vp, _vp, _c_i64, _c_i64,
                                     _vp, _vp, _c_i64, _c_i64, _vp, _vp, _vp, _vp, _vp, _vp,
                                     ctypes.c_size_t, _vp]),
+    "sldm_layer_norm_fwd": (ctypes.c_int, [ctypes.c_int, _vp, _c_i64, _c_i64, _c_i64, _vp, _vp,
+                                           ctypes.c_float, _vp, _vp, _vp, _vp]),
+    "sldm_layer_norm_bwd_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int, _c_i64, _c_i64]),
+    "sldm_layer_norm_bwd": (ctypes.c_int, [ctypes.c_int, _vp, _c_i64, _vp, _c_i64, _c_i64, _c_i64,
+                                           _vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t,
+                                           _vp]),
+    "sldm_rotary_axes": (ctypes.c_int, [ctypes.c_int, _vp, _vp, _c_i64, _vp, _vp, _c_i64, _c_i64,
+                                        _c_i64, _c_i64, _vp, ctypes.c_int, _vp, _vp, _vp, _c_i64,
+                                        ctypes.c_int, ctypes.c_int, _vp, _vp, _vp]),
+    "sldm_decay_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int, _c_i64, _c_i64,
+                                                               _c_i64, _c_i64, _c_i64, _c_i64,
+                                                               ctypes.c_int]),
+    "sldm_decay_attention_fwd": (ctypes.c_int, [ctypes.c_int, _vp, _vp, _vp, _vp, _vp, _vp, _c_i64,
+                                                _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp,
+                                                ctypes.c_float, _vp, _vp, ctypes.c_int, _vp, _vp,
+                                                _vp, ctypes.c_size_t, _vp]),
+    "sldm_decay_attention_bwd": (ctypes.c_int, [ctypes.c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                                _vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,
+                                                _c_i64, _vp, ctypes.c_float, _vp, _vp, _vp,
+                                                ctypes.c_int, _vp, _vp, _vp, _vp, _vp,
+                                                ctypes.c_size_t, _vp]),
+    "sldm_decay_attention_step": (ctypes.c_int, [ctypes.c_int, _vp, _vp, _vp, _vp, _vp, _vp,
+                                                 _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp,
+                                                 ctypes.c_float, _vp, _vp, _vp]),
 }
 
 _lock = threading.Lock()
