@@ -11,7 +11,7 @@ namespace {
 constexpr int kMaxDim = 128;
 constexpr int64_t kMaxThreads = (int64_t)1 << 32;   // work-items of one launch, exclusive
 
-int chunk_of(int dtype) { return dtype == SLDM_F32 ? 32 : 64; }
+int chunk_of(int dtype) { return dtype == SLDM_F32 ? 16 : 64; }
 
 // Segments of the time axis.  One workgroup walks a sequence alone unless that
 // leaves the chip short of waves (256 CUs x 4 SIMDs x 2); then the axis is cut
