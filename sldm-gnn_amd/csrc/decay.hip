@@ -11,7 +11,7 @@ namespace {
 constexpr int kMaxDim = 128;
 constexpr int64_t kMaxThreads = (int64_t)1 << 32;   // work-items of one launch, exclusive
 
-int chunk_of(int dtype) { return dtype == SLDM_F32 ? 16 : 64; }
+int chunk_of(int dtype) { return dtype == SLDM_F32 ? 16 : 32; }
 
 // Segments of the time axis.  One workgroup walks a sequence alone unless that
 // leaves the chip short of waves (256 CUs x 4 SIMDs x 2); then the axis is cut
@@ -163,7 +163,7 @@ void launch_roles(int dtype, Args& a, const Role* const* roles, int n, bool out,
     if (done[i]) continue;
     int m = 0;
     for (int j = i; j < n; ++j)
-      if (!done[j] && tiles_of(roles[j]->kd) == tiles_of(roles[i]->kd) &&
+      if (!done[j] && row_tiles(roles[j]->kd) == row_tiles(roles[i]->kd) &&
           tiles_of(roles[j]->vd) == tiles_of(roles[i]->vd)) {
         a.role[m++] = *roles[j];
         done[j] = true;

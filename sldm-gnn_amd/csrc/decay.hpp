@@ -102,6 +102,7 @@ __device__ __forceinline__ Span span_of(const Args& a, const Role& R, int id) {
 // out: roles write outputs; else states only.  wave_cols: value columns a wave owns.
 void run_bf16(const Args& a, int roles, bool out, hipStream_t stream);
 void run_f32(const Args& a, int roles, bool out, hipStream_t stream);
-inline int tiles_of(int d) { return d <= 32 ? 1 : d <= 64 ? 2 : 4; }
+inline int tiles_of(int d) { return d <= 32 ? 1 : d <= 64 ? 2 : 4; }   // waves across vd
+inline int row_tiles(int d) { return (d + 31) / 32; }
 
 }  // namespace sldm_decay

@@ -1,0 +1,415 @@
+// Decay attention in bf16 (mathematics: decay.hpp), kernel: chunks of 32 tokens on
+// v_mfma_f32_32x32x16_bf16, fp32 accumulation.
+//
+// A workgroup owns one (batch, head, segment); a wave owns 32 value columns and
+// keeps its Dk x 32 slice of the state in accumulators for the whole walk.  Q, K
+// and V tiles come by LDS-DMA (no registers on the way) into two buffers, the
+// next chunk's while this one is computed, with one barrier a chunk; an output
+// chunk is stored behind the next barrier, so that its stores have a chunk's time
+// before anything waits for memory.  The 16-byte granules of a row are
+// XOR-swizzled through the DMA's source addresses, so that row reads (one granule
+// of eight rows) and transposed reads (ds_read_b64_tr_b16: 64 bytes of four rows)
+// spread over the banks.  Chunks of 64 (half as many state conversions) were
+// slower: their tiles and accumulators leave two waves a SIMD and spill.
+//
+// Roundings.  The state is held in fp32 and read as bf16, and P = Q K^T o D is
+// rounded to bf16: the products of an output are each off by at most 2^-8 of
+// themselves, at random, and together by about what rounding the output costs
+// (relative error 0.0024 with both, 0.0017 for the rounding of the output alone).
+// The state's update takes V g^{n-1-j} as hi + mid (16 significant bits).  Where
+// the walk's state is an output, in fp32, it takes hi + mid + lo (all 24), and P
+// goes in as hi + lo; so in short sequences, whose outputs hang on few entries of
+// P, which do not average out.  (Both in one kernel, chosen by a branch, spill.)
+#pragma once
+
+#include "decay.hpp"
+
+namespace sldm_decay {
+namespace {
+
+typedef __bf16 bf8v __attribute__((ext_vector_type(8)));
+typedef short s4v __attribute__((ext_vector_type(4)));
+typedef short s8v __attribute__((ext_vector_type(8)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) void* lds_vptr;
+constexpr int C = 32;
+constexpr int kShort = 128;      // tokens of a sequence that counts as short
+
+__device__ __forceinline__ f16v mfma(bf8v a, bf8v b, f16v c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ bf8v as_bf8(sldm::bf16x8 v) { return __builtin_bit_cast(bf8v, v); }
+__device__ __forceinline__ bf8v pack8(const float (&v)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = sldm::pack_bf16x2(v[2 * e], v[2 * e + 1]);
+  return __builtin_bit_cast(bf8v, make_uint4(w[0], w[1], w[2], w[3]));
+}
+
+// LDS rows of 32 DT values (96 take the room of 128) and their swizzle: granule g
+// of row r lies at g ^ swz(r).  Four neighbouring rows' transposed reads fall into
+// the four quarters of the banks, eight rows' granules into eight places.
+constexpr int row_bytes(int dt) { return dt == 1 ? 64 : dt == 2 ? 128 : 256; }
+template <int RB>
+__device__ __forceinline__ int swz(int r) {
+  const int low = ((r >> 2) & 1) | ((r >> 2) & 2);
+  return RB == 64 ? low : RB == 128 ? ((r & 2) << 1) | low : ((r & 3) << 2) | low;
+}
+
+// A tile of C rows by LDS-DMA: 64 granules an instruction, instruction i of the
+// tile by wave i % NW.  Lanes without a source (columns past d, rows in front of
+// the segment) stay out and leave their place as it is: zeros, written once.
+template <int DT, int NW>
+struct Tile {
+  static constexpr int RB = row_bytes(DT), GR = RB / 16, BYTES = C * RB, INSTR = BYTES / 1024;
+  static constexpr int N = (INSTR + NW - 1) / NW, ROWS = 64 / GR;
+  const char* base;        // of the lowest-addressed row of chunk 0
+  int64_t step;            // bytes from chunk to chunk
+  uint32_t voff[N];
+  uint32_t on;             // bit i: this lane takes part in instruction i
+  __device__ __forceinline__ void init(const Operand& t, const uint16_t* head, const Span& s, int64_t sign, int pad,
+                                       int d, int wave, int lane) {
+    const int64_t st = t.st;
+    base = reinterpret_cast<const char*>(head + (s.base - sign * pad + (sign < 0 ? -(C - 1) : 0)) * st);
+    step = sign * C * st * 2;
+    on = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = (i * NW + wave) * ROWS + lane / GR, g = lane % GR ^ swz<RB>(r);
+      voff[i] = (uint32_t)((sign < 0 ? C - 1 - r : r) * st * 2) + 16 * g;
+      on |= (i * NW + wave < INSTR && 8 * g < d ? 1u : 0u) << i;
+    }
+  }
+  // rows from `first` on
+  __device__ __forceinline__ void load(int64_t c, uint32_t lds, int first, int wave, int lane) const {
+    const char* p = base + c * step;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t at = lds + (uint32_t)((i * NW + wave) * 1024);
+      if ((on >> i & 1) && (i * NW + wave) * ROWS + lane / GR >= first)
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                     :: "v"(voff[i]), "s"(p), "s"(__builtin_amdgcn_readfirstlane(at)) : "memory", "m0");
+    }
+  }
+};
+// Any alignment: element by element.
+template <int DT, int NTH>
+__device__ __forceinline__ void tile_slow(char* lds, const uint16_t* row0, int64_t st, int64_t x0, int d) {
+  constexpr int RB = row_bytes(DT);
+#pragma unroll 1
+  for (int i = threadIdx.x; i < C * DT * 32; i += NTH) {
+    const int r = i / (DT * 32), e = i % (DT * 32);
+    const int64_t x = x0 + r;
+    *reinterpret_cast<uint16_t*>(lds + r * RB + ((e / 8 ^ swz<RB>(r)) << 4) + 2 * (e % 8)) =
+        x >= 0 && e < d ? row0[x * st + e] : (uint16_t)0;
+  }
+}
+
+// lane -> column (or row) inside a 32-wide tile: the middle two bits of each
+// 16-group swapped, which makes the accumulator rows 8 s .. 8 s + 7 of a half
+// wave eight neighbours: 16 s + 8 h + e.
+__device__ __forceinline__ int perm16(int m) { return (m & ~12) | ((m & 4) << 1) | ((m & 8) >> 1); }
+
+// Operand whose rows are a tile's rows: lane `row`, columns 16 t + 8 h .. + 7.
+struct RowRead {
+  uint32_t base, x;
+  template <int RB>
+  __device__ __forceinline__ void init(int row, int h) {
+    base = row * RB;
+    x = (h ^ swz<RB>(row)) << 4;
+  }
+  __device__ __forceinline__ bf8v at(const char* lds, int t) const {
+    return *reinterpret_cast<const bf8v*>(lds + base + (x ^ (32 * t)));
+  }
+};
+// Operand whose rows are a tile's columns: lane m holds column 32 ct + perm16(m)
+// of the eight rows 16 s + 8 h ..
+struct ColRead {
+  uint32_t base, x;
+  template <int RB>
+  __device__ __forceinline__ void init(int lane) {
+    const int q = lane >> 4, r16 = lane & 15, blk = r16 & 3, b = ((blk & 1) << 1) | (blk >> 1);
+    const int row = 8 * (q >> 1) + (r16 >> 2);
+    base = row * RB + 8 * (b & 1);
+    x = ((2 * (q & 1) + (b >> 1)) ^ swz<RB>(row)) << 4;
+  }
+  template <int RB>
+  __device__ __forceinline__ bf8v at(const char* lds, int ct, int s) const {
+    typedef __attribute__((address_space(3))) s4v* lp;
+    const char* p = lds + base + 16 * s * RB;      // rows + 4: bit 0 of the swizzle flips
+    const s4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p + (x ^ (64 * ct))));
+    const s4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p + 4 * RB + (x ^ (64 * ct) ^ 16)));
+    return __builtin_bit_cast(bf8v, s8v{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+  }
+};
+
+// Instructions stay on their side: scheduled over a whole chunk, the operands of
+// all products are in registers at once and spill.
+__device__ __forceinline__ void phase() { __builtin_amdgcn_sched_barrier(0); }
+
+// The state's update: S <- g^n S + K^T diag(w) V, V diag(w) in TERMS parts.
+template <int KT, int TERMS>
+__device__ __forceinline__ void update(f16v (&S)[KT], const bf8v (&vf)[2], const char* lk, const ColRead& ck,
+                                       const float* pw, float gn) {
+#pragma unroll
+  for (int t = 0; t < KT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) S[t][r] *= gn;
+  bf8v kn = ck.at<row_bytes(KT)>(lk, 0, 0);
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const float* w = pw + 16 * s;
+    const uint4 u = __builtin_bit_cast(uint4, vf[s]);
+    const float x[8] = {sldm::bf16_lo(u.x) * w[0], sldm::bf16_hi(u.x) * w[1], sldm::bf16_lo(u.y) * w[2],
+                        sldm::bf16_hi(u.y) * w[3], sldm::bf16_lo(u.z) * w[4], sldm::bf16_hi(u.z) * w[5],
+                        sldm::bf16_lo(u.w) * w[6], sldm::bf16_hi(u.w) * w[7]};
+    sldm::bf16x8 hi, mid, lo;
+    if constexpr (TERMS == 3) sldm::split3_bf16x8(x, hi, mid, lo);
+    else sldm::split_bf16x8(x, hi, mid);
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      const bf8v kf = kn;
+      if (s * KT + t + 1 < 2 * KT) kn = ck.at<row_bytes(KT)>(lk, (t + 1) % KT, s + (t + 1) / KT);
+      if constexpr (TERMS == 3) S[t] = mfma(kf, as_bf8(lo), S[t]);
+      S[t] = mfma(kf, as_bf8(mid), S[t]);
+      S[t] = mfma(kf, as_bf8(hi), S[t]);
+      phase();
+    }
+  }
+}
+
+// OUT: outputs, else the state alone.  EXACT: the roundings of a short sequence or
+// an output state (above).  FAST: by Tile, else by tile_slow.
+template <int KT, int NW, bool OUT, bool EXACT, bool FAST>
+__global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_bf16_kernel(Args a) {
+  using TK = Tile<KT, NW>;
+  using TV = Tile<NW, NW>;
+  constexpr int NTH = 64 * NW, RBK = TK::RB, RBV = TV::RB;
+  constexpr int kBuf = TK::BYTES * (OUT ? 2 : 1) + TV::BYTES;       // k, v, q
+  __shared__ __attribute__((aligned(1024))) char tiles[2 * kBuf];
+  __shared__ __attribute__((aligned(16))) float wtab[C], dtab[2 * C];
+
+  const int id = xcd_order();
+  if (id >= a.groups) return;
+  const Role& R = a.role[blockIdx.y];
+  const Span sp = span_of(a, R, id);
+  const int seg = (int)(sp.seg0 / a.seg_len);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int m = lane & 31, h = lane >> 5;
+  const int kd = R.kd, vd = R.vd;
+  const int pad = (int)((C - sp.n % C) % C);
+  const int64_t nch = (sp.n + pad) / C;
+  const float ld2 = a.log_decay[sp.hd] * 1.44269504088896340736f;
+  const int64_t sign = R.reverse ? -1 : 1;
+
+  const uint16_t* qh = OUT ? reinterpret_cast<const uint16_t*>(R.q.p) + sp.b * R.q.sb + (sp.hd / R.q.hdiv) * R.q.sh : nullptr;
+  const uint16_t* kh = reinterpret_cast<const uint16_t*>(R.k.p) + sp.b * R.k.sb + (sp.hd / R.k.hdiv) * R.k.sh;
+  const uint16_t* vh = reinterpret_cast<const uint16_t*>(R.v.p) + sp.b * R.v.sb + (sp.hd / R.v.hdiv) * R.v.sh;
+
+  TK tq, tk;
+  TV tv;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_vptr)tiles;
+  auto fetch = [&](int64_t c, int first) {
+    const uint32_t at = lds0 + (uint32_t)(c & 1) * kBuf;
+    tk.load(c, at, first, wave, lane);
+    tv.load(c, at + TK::BYTES, first, wave, lane);
+    if constexpr (OUT) tq.load(c, at + TK::BYTES + TV::BYTES, first, wave, lane);
+  };
+  if (FAST && nch > 0) {
+    if (pad > 0 || kd < 32 * KT || vd < 32 * NW) {
+      for (int i = threadIdx.x; i < 2 * kBuf / 16; i += NTH) reinterpret_cast<uint4*>(tiles)[i] = make_uint4(0, 0, 0, 0);
+      __syncthreads();
+    }
+    tk.init(R.k, kh, sp, sign, pad, kd, wave, lane);
+    tv.init(R.v, vh, sp, sign, pad, vd, wave, lane);
+    if constexpr (OUT) tq.init(R.q, qh, sp, sign, pad, kd, wave, lane);
+    fetch(0, pad);
+  }
+  // state: lane = value column, register 8 s + e of tile t = row 32 t + 16 s + 8 h + e
+  const int vc = 32 * wave + perm16(m);
+  f16v S[KT];
+#pragma unroll
+  for (int t = 0; t < KT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) S[t][r] = 0.f;
+  if (R.s0) {
+    const float* s0 = R.s0 + sp.bh * R.s0_bh + seg * R.s0_seg;
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int kr = 32 * t + 16 * (r >> 3) + 8 * h + (r & 7);
+        if (kr < kd && vc < vd) S[t][r] = s0[kr * R.s_k + vc * R.s_v];
+      }
+  }
+  // wtab[j]: the weight with which row j enters the state; dtab[32 + i - j]: D
+  for (int j = threadIdx.x; j < C; j += NTH) wtab[j] = powg(ld2, C - 1 - j + R.delta) * R.upd_scale;
+  for (int j = threadIdx.x; j < 2 * C; j += NTH) dtab[j] = j < C ? 0.f : powg(ld2, j - C) * R.p_scale;
+
+  RowRead rq, rk;
+  ColRead ck, cv;
+  rq.init<RBK>(m, h);
+  rk.init<RBK>(perm16(m), h);
+  ck.init<RBK>(lane);
+  cv.init<RBV>(lane);
+  const float* pd = dtab + 9 + m - 8 * h;                       // + 23 - (16 s + e): entry 32 + m - j
+  const float* pw = wtab + 8 * h;
+  f16v O;
+  // chunk c's outputs: lane = token m, registers 8 s + e = columns 16 s + 8 h + e
+  auto put = [&](int64_t c) {
+    const int64_t x = c * C + m - pad;
+    if (x < 0) return;
+    const int64_t off = sp.b * R.o_sb + (sp.base + sign * x) * R.o_st + sp.hd * R.o_sh + 32 * wave + 8 * h;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int c0 = 32 * wave + 16 * s + 8 * h;
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = O[8 * s + e];
+      if (R.o_f32) {
+        float* o = reinterpret_cast<float*>(R.o) + off + 16 * s;
+        if (FAST) {
+          if (c0 < vd) {
+            sldm::Vec<float, 4>::store(o, y);
+            sldm::Vec<float, 4>::store(o + 4, y + 4);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (c0 + e < vd) o[e] = y[e];
+        }
+      } else {
+        uint16_t* o = reinterpret_cast<uint16_t*>(R.o) + off + 16 * s;
+        if (FAST) {
+          if (c0 < vd) sldm::Vec<uint16_t, 8>::store(o, y);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (c0 + e < vd) o[e] = sldm::f32_to_bf16(y[e]);
+        }
+      }
+    }
+  };
+
+  for (int64_t c = 0; c < nch; ++c) {
+    if constexpr (FAST) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // this chunk's tiles (and older stores)
+      __syncthreads();                                          // of all waves; the other buffer is free
+      if (OUT && c > 0) put(c - 1);
+      if (c + 1 < nch) fetch(c + 1, 0);
+    } else {
+      if (OUT && c > 0) put(c - 1);
+      __syncthreads();
+      const int64_t x0 = c * C - pad;
+      char* at = tiles + (c & 1) * kBuf;
+      tile_slow<KT, NTH>(at, kh + sp.base * R.k.st, sign * R.k.st, x0, kd);
+      tile_slow<NW, NTH>(at + TK::BYTES, vh + sp.base * R.v.st, sign * R.v.st, x0, vd);
+      if constexpr (OUT) tile_slow<KT, NTH>(at + TK::BYTES + TV::BYTES, qh + sp.base * R.q.st, sign * R.q.st, x0, kd);
+      __syncthreads();
+    }
+    // the tables are read, and the operands' places worked out, anew: not kept in registers
+    asm volatile("" : "+v"(rq.x), "+v"(rk.x), "+v"(ck.x), "+v"(cv.x) :: "memory");
+    const char* lk = tiles + (c & 1) * kBuf;
+    const char* lv = lk + TK::BYTES;
+    const char* lq = lv + TV::BYTES;
+    const int padc = c == 0 ? pad : 0;
+    bf8v vf[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) vf[s] = cv.at<RBV>(lv, wave, s);
+    if constexpr (OUT) {
+      f16v P;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) O[r] = P[r] = 0.f;
+      bf8v qn = rq.at(lq, 0), kn = rk.at(lk, 0);
+#pragma unroll
+      for (int t = 0; t < 2 * KT; ++t) {
+        const bf8v qf = qn, kf = kn;
+        if (t + 1 < 2 * KT) {
+          qn = rq.at(lq, t + 1);
+          kn = rk.at(lk, t + 1);
+        }
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = S[t >> 1][8 * (t & 1) + e];
+        O = mfma(pack8(x), qf, O);
+        P = mfma(kf, qf, P);
+        phase();
+      }
+      const float rd = powg(ld2, m - padc + 1 - R.delta) * R.read_scale;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) O[r] *= rd;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = P[8 * s + e] * pd[23 - 16 * s - e];
+        if constexpr (EXACT) {
+          sldm::bf16x8 hi, lo;
+          sldm::split_bf16x8(x, hi, lo);
+          O = mfma(vf[s], as_bf8(lo), O);
+          O = mfma(vf[s], as_bf8(hi), O);
+        } else {
+          O = mfma(vf[s], pack8(x), O);
+        }
+      }
+    }
+    const float gn = powg(ld2, C - padc);
+    update<KT, EXACT ? 3 : 2>(S, vf, lk, ck, pw, gn);
+  }
+  if (OUT && nch > 0) put(nch - 1);
+  if (R.s1) {
+    float* s1 = R.s1 + sp.bh * R.s1_bh + seg * R.s1_seg;
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int kr = 32 * t + 16 * (r >> 3) + 8 * h + (r & 7);
+        if (kr < kd && vc < vd) s1[kr * R.s_k + vc * R.s_v] = S[t][r];
+      }
+  }
+  if constexpr (OUT) {                                          // tokens behind the sequence's end: zeros
+    const int64_t t1 = sp.seg0 + a.seg_len < a.T ? sp.seg0 + a.seg_len : a.T;
+    const int64_t t0 = sp.len > sp.seg0 ? sp.len : sp.seg0;
+    const int64_t todo = t1 > t0 ? (t1 - t0) * vd : 0;
+    for (int64_t i = threadIdx.x; i < todo; i += NTH) {
+      const int64_t off = sp.b * R.o_sb + (t0 + i / vd) * R.o_st + sp.hd * R.o_sh + i % vd;
+      if (R.o_f32) reinterpret_cast<float*>(R.o)[off] = 0.f;
+      else reinterpret_cast<uint16_t*>(R.o)[off] = 0;
+    }
+  }
+}
+
+template <int KT, int NW, bool OUT, bool EXACT, bool FAST = true>
+void launch(const Args& a, int roles, hipStream_t st) {
+  decay_bf16_kernel<KT, NW, OUT, EXACT, FAST>
+      <<<dim3((unsigned)((a.groups + 7) / 8 * 8), roles), 64 * NW, 0, st>>>(a);
+}
+template <int KT, bool OUT, bool EXACT>
+void by_cols(const Args& a, int nw, int roles, hipStream_t st) {
+  if (nw == 1) launch<KT, 1, OUT, EXACT>(a, roles, st);
+  else if (nw == 2) launch<KT, 2, OUT, EXACT>(a, roles, st);
+  else launch<KT, 4, OUT, EXACT>(a, roles, st);
+}
+template <bool OUT, bool EXACT>
+void by_rows(const Args& a, int roles, hipStream_t st) {
+  const int kt = row_tiles(a.role[0].kd), nw = tiles_of(a.role[0].vd);
+  if (kt == 1) by_cols<1, OUT, EXACT>(a, nw, roles, st);
+  else if (kt == 2) by_cols<2, OUT, EXACT>(a, nw, roles, st);
+  else if (kt == 3) by_cols<3, OUT, EXACT>(a, nw, roles, st);
+  else by_cols<4, OUT, EXACT>(a, nw, roles, st);
+}
+// Rows of a chunk within 32-bit byte offsets of each other.
+inline bool near(const Operand& t) { return t.st >= 0 && t.st < ((int64_t)1 << 25); }
+// Every operand's rows on 16-byte boundaries and whole granules.
+inline bool all_fast(const Args& a, int roles, bool out) {
+  bool ok = true;
+  for (int i = 0; i < roles; ++i) {
+    const Role& r = a.role[i];
+    ok = ok && r.k.vec && r.v.vec && r.kd % 8 == 0 && r.vd % 8 == 0 && (!out || (r.q.vec && r.o_vec)) &&
+         near(r.k) && near(r.v) && (!out || near(r.q));
+  }
+  return ok;
+}
+
+}  // namespace
+}  // namespace sldm_decay

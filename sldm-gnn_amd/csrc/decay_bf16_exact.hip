@@ -1,0 +1,7 @@
+// bf16 instances of the decay attention kernel: short sequences, and walks whose
+// state is an output.
+#include "decay_bf16.hpp"
+
+namespace sldm_decay {
+void run_bf16_exact(const Args& a, int roles, hipStream_t st) { by_rows<true, true>(a, roles, st); }
+}  // namespace sldm_decay
