@@ -58,6 +58,7 @@ struct Args {
   Role role[3];
   int64_t B, H, T, seg_len;
   int nseg, groups;     // groups = B H nseg
+  int roles;
   const float* log_decay;
   const void* lengths;  // null: T each
   int lengths64;
@@ -72,9 +73,9 @@ __device__ __forceinline__ int64_t seq_len(const Args& a, int64_t b) {
   return n < 0 ? 0 : (n > a.T ? a.T : n);
 }
 
-// Workgroups are dealt to the XCDs in turn; neighbours in (segment, batch, head)
-// order, whose rows share cache lines, are put on one XCD.  gridDim.x is a
-// multiple of 8.
+// Workgroups are dealt to the XCDs in turn; neighbours in (segment, batch, head,
+// role) order are put on one XCD: heads share cache lines, and the roles of one
+// head read the same tensors.  gridDim.x is a multiple of 8.
 __device__ __forceinline__ int xcd_order() {
   return ((int)blockIdx.x & 7) * ((int)gridDim.x >> 3) + ((int)blockIdx.x >> 3);
 }
@@ -98,10 +99,79 @@ __device__ __forceinline__ Span span_of(const Args& a, const Role& R, int id) {
   return s;
 }
 
-// One launch of `roles` roles whose kd and vd fall into the same tile classes.
-// out: roles write outputs; else states only.  wave_cols: value columns a wave owns.
-void run_bf16(const Args& a, int roles, bool out, hipStream_t stream);
-void run_f32(const Args& a, int roles, bool out, hipStream_t stream);
+typedef __attribute__((address_space(3))) void* lds_vptr;
+
+// A tile of ROWS rows of RB bytes in LDS, by LDS-DMA: 64 granules of 16 bytes an
+// instruction, instruction i of the tile by wave i % NW; granule g of row r lies
+// at g ^ SWZ<RB>::of(r), by choice of the source address.  Lanes without a source
+// (columns past d, rows in front of the segment) stay out and leave their place
+// as it is: zeros, written once.
+template <typename T, int ROWS, int RB, int NW, template <int> class SWZ>
+struct Tile {
+  static constexpr int kRB = RB, GR = RB / 16, BYTES = ROWS * RB, INSTR = BYTES / 1024, E = 16 / (int)sizeof(T);
+  static constexpr int N = (INSTR + NW - 1) / NW, STEP = 64 / GR;
+  static_assert(BYTES % 1024 == 0 && GR <= 64, "whole instructions");
+  const char* base;        // of the lowest-addressed row of chunk 0
+  int64_t step;            // bytes from chunk to chunk
+  uint32_t voff[N];
+  uint32_t on;             // bit i: this lane takes part in instruction i
+  static __device__ __forceinline__ int row_of(int i) {
+    return (i * NW + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * STEP + (int)(threadIdx.x & 63) / GR;
+  }
+  __device__ __forceinline__ void init(const Operand& t, const T* head, const Span& s, int64_t sign, int pad, int d) {
+    const int64_t st = t.st;
+    base = reinterpret_cast<const char*>(head + (s.base - sign * pad + (sign < 0 ? -(ROWS - 1) : 0)) * st);
+    step = sign * ROWS * st * (int)sizeof(T);
+    on = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = row_of(i), g = (int)(threadIdx.x & 63) % GR ^ SWZ<RB>::of(r);
+      voff[i] = (uint32_t)((sign < 0 ? ROWS - 1 - r : r) * st * (int)sizeof(T)) + 16 * g;
+      on |= (r < ROWS && E * g < d ? 1u : 0u) << i;
+    }
+  }
+  // chunk c, rows from `first` on, to LDS address `lds`
+  __device__ __forceinline__ void load(int64_t c, uint32_t lds, int first) const {
+    const char* p = base + c * step;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if ((on >> i & 1) && row_of(i) >= first)
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                     :: "v"(voff[i]), "s"(p), "s"(__builtin_amdgcn_readfirstlane(lds + (uint32_t)((i * NW + wave) * 1024)))
+                     : "memory", "m0");
+  }
+  // any alignment: element by element; row r is position x0 + r (below 0: zeros)
+  static __device__ __forceinline__ void slow(char* lds, const T* row0, int64_t st, int64_t x0, int d) {
+    constexpr int W = RB / (int)sizeof(T);
+#pragma unroll 1
+    for (int i = threadIdx.x; i < ROWS * W; i += 64 * NW) {
+      const int r = i / W, e = i % W;
+      const int64_t x = x0 + r;
+      *reinterpret_cast<T*>(lds + r * RB + ((e / E ^ SWZ<RB>::of(r)) << 4) + (int)sizeof(T) * (e % E)) =
+          x >= 0 && e < d ? row0[x * st + e] : T(0);
+    }
+  }
+};
+
+// Rows of a chunk within 32-bit byte offsets of each other.
+inline bool near(const Operand& t) { return t.st >= 0 && t.st < ((int64_t)1 << 24); }
+// Whether every operand can come by DMA: rows on 16-byte boundaries, whole granules.
+inline bool all_fast(const Args& a, bool out, int granule) {
+  bool ok = true;
+  for (int i = 0; i < a.roles; ++i) {
+    const Role& r = a.role[i];
+    ok = ok && r.k.vec && r.v.vec && r.kd % granule == 0 && r.vd % granule == 0 && near(r.k) && near(r.v) &&
+         (!out || (r.q.vec && r.o_vec && near(r.q)));
+  }
+  return ok;
+}
+
+// One launch of roles whose kd and vd fall into the same tile classes.
+// out: roles write outputs; else states only.
+void run_bf16(const Args& a, bool out, hipStream_t stream);
+void run_f32(const Args& a, bool out, hipStream_t stream);
+inline unsigned grid_of(const Args& a) { return (unsigned)(((int64_t)a.groups * a.roles + 7) / 8 * 8); }
 inline int tiles_of(int d) { return d <= 32 ? 1 : d <= 64 ? 2 : 4; }   // waves across vd
 inline int row_tiles(int d) { return (d + 31) / 32; }
 

@@ -4,20 +4,20 @@
 
 namespace sldm_decay {
 
-void run_bf16_exact(const Args& a, int roles, hipStream_t st);
+void run_bf16_exact(const Args& a, hipStream_t st);
 
-void run_bf16(const Args& a, int roles, bool out, hipStream_t st) {
+void run_bf16(const Args& a, bool out, hipStream_t st) {
   bool exact = a.T <= kShort;
-  for (int i = 0; i < roles; ++i) exact = exact || a.role[i].s1;
-  if (!all_fast(a, roles, out)) {
-    if (out) launch<4, 4, true, true, false>(a, roles, st);
-    else launch<4, 4, false, true, false>(a, roles, st);
+  for (int i = 0; i < a.roles; ++i) exact = exact || a.role[i].s1;
+  if (!all_fast(a, out, 8)) {
+    if (out) launch<4, 4, true, true, false>(a, st);
+    else launch<4, 4, false, true, false>(a, st);
   } else if (!out) {
-    by_rows<false, true>(a, roles, st);
+    by_rows<false, true>(a, st);
   } else if (exact) {
-    run_bf16_exact(a, roles, st);
+    run_bf16_exact(a, st);
   } else {
-    by_rows<true, false>(a, roles, st);
+    by_rows<true, false>(a, st);
   }
 }
 

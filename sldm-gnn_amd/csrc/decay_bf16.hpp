@@ -31,7 +31,6 @@ typedef __bf16 bf8v __attribute__((ext_vector_type(8)));
 typedef short s4v __attribute__((ext_vector_type(4)));
 typedef short s8v __attribute__((ext_vector_type(8)));
 typedef float f16v __attribute__((ext_vector_type(16)));
-typedef __attribute__((address_space(3))) void* lds_vptr;
 constexpr int C = 32;
 constexpr int kShort = 128;      // tokens of a sequence that counts as short
 
@@ -46,64 +45,18 @@ __device__ __forceinline__ bf8v pack8(const float (&v)[8]) {
   return __builtin_bit_cast(bf8v, make_uint4(w[0], w[1], w[2], w[3]));
 }
 
-// LDS rows of 32 DT values (96 take the room of 128) and their swizzle: granule g
-// of row r lies at g ^ swz(r).  Four neighbouring rows' transposed reads fall into
-// the four quarters of the banks, eight rows' granules into eight places.
+// LDS rows of 32 DT values (96 take the room of 128); swizzle: granule g of row r
+// lies at g ^ swz(r).  Four neighbouring rows' transposed reads (64 bytes of
+// each) fall into the four quarters of the banks, eight rows' granules into eight
+// places.
 constexpr int row_bytes(int dt) { return dt == 1 ? 64 : dt == 2 ? 128 : 256; }
 template <int RB>
-__device__ __forceinline__ int swz(int r) {
-  const int low = ((r >> 2) & 1) | ((r >> 2) & 2);
-  return RB == 64 ? low : RB == 128 ? ((r & 2) << 1) | low : ((r & 3) << 2) | low;
-}
-
-// A tile of C rows by LDS-DMA: 64 granules an instruction, instruction i of the
-// tile by wave i % NW.  Lanes without a source (columns past d, rows in front of
-// the segment) stay out and leave their place as it is: zeros, written once.
-template <int DT, int NW>
-struct Tile {
-  static constexpr int RB = row_bytes(DT), GR = RB / 16, BYTES = C * RB, INSTR = BYTES / 1024;
-  static constexpr int N = (INSTR + NW - 1) / NW, ROWS = 64 / GR;
-  const char* base;        // of the lowest-addressed row of chunk 0
-  int64_t step;            // bytes from chunk to chunk
-  uint32_t voff[N];
-  uint32_t on;             // bit i: this lane takes part in instruction i
-  __device__ __forceinline__ void init(const Operand& t, const uint16_t* head, const Span& s, int64_t sign, int pad,
-                                       int d, int wave, int lane) {
-    const int64_t st = t.st;
-    base = reinterpret_cast<const char*>(head + (s.base - sign * pad + (sign < 0 ? -(C - 1) : 0)) * st);
-    step = sign * C * st * 2;
-    on = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int r = (i * NW + wave) * ROWS + lane / GR, g = lane % GR ^ swz<RB>(r);
-      voff[i] = (uint32_t)((sign < 0 ? C - 1 - r : r) * st * 2) + 16 * g;
-      on |= (i * NW + wave < INSTR && 8 * g < d ? 1u : 0u) << i;
-    }
-  }
-  // rows from `first` on
-  __device__ __forceinline__ void load(int64_t c, uint32_t lds, int first, int wave, int lane) const {
-    const char* p = base + c * step;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const uint32_t at = lds + (uint32_t)((i * NW + wave) * 1024);
-      if ((on >> i & 1) && (i * NW + wave) * ROWS + lane / GR >= first)
-        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
-                     :: "v"(voff[i]), "s"(p), "s"(__builtin_amdgcn_readfirstlane(at)) : "memory", "m0");
-    }
+struct Swizzle {
+  static __device__ __forceinline__ int of(int r) {
+    const int low = ((r >> 2) & 1) | ((r >> 2) & 2);
+    return RB == 64 ? low : RB == 128 ? ((r & 2) << 1) | low : ((r & 3) << 2) | low;
   }
 };
-// Any alignment: element by element.
-template <int DT, int NTH>
-__device__ __forceinline__ void tile_slow(char* lds, const uint16_t* row0, int64_t st, int64_t x0, int d) {
-  constexpr int RB = row_bytes(DT);
-#pragma unroll 1
-  for (int i = threadIdx.x; i < C * DT * 32; i += NTH) {
-    const int r = i / (DT * 32), e = i % (DT * 32);
-    const int64_t x = x0 + r;
-    *reinterpret_cast<uint16_t*>(lds + r * RB + ((e / 8 ^ swz<RB>(r)) << 4) + 2 * (e % 8)) =
-        x >= 0 && e < d ? row0[x * st + e] : (uint16_t)0;
-  }
-}
 
 // lane -> column (or row) inside a 32-wide tile: the middle two bits of each
 // 16-group swapped, which makes the accumulator rows 8 s .. 8 s + 7 of a half
@@ -116,7 +69,7 @@ struct RowRead {
   template <int RB>
   __device__ __forceinline__ void init(int row, int h) {
     base = row * RB;
-    x = (h ^ swz<RB>(row)) << 4;
+    x = (h ^ Swizzle<RB>::of(row)) << 4;
   }
   __device__ __forceinline__ bf8v at(const char* lds, int t) const {
     return *reinterpret_cast<const bf8v*>(lds + base + (x ^ (32 * t)));
@@ -131,7 +84,7 @@ struct ColRead {
     const int q = lane >> 4, r16 = lane & 15, blk = r16 & 3, b = ((blk & 1) << 1) | (blk >> 1);
     const int row = 8 * (q >> 1) + (r16 >> 2);
     base = row * RB + 8 * (b & 1);
-    x = ((2 * (q & 1) + (b >> 1)) ^ swz<RB>(row)) << 4;
+    x = ((2 * (q & 1) + (b >> 1)) ^ Swizzle<RB>::of(row)) << 4;
   }
   template <int RB>
   __device__ __forceinline__ bf8v at(const char* lds, int ct, int s) const {
@@ -151,11 +104,9 @@ __device__ __forceinline__ void phase() { __builtin_amdgcn_sched_barrier(0); }
 template <int KT, int TERMS>
 __device__ __forceinline__ void update(f16v (&S)[KT], const bf8v (&vf)[2], const char* lk, const ColRead& ck,
                                        const float* pw, float gn) {
+  bf8v kf[2][KT];
 #pragma unroll
-  for (int t = 0; t < KT; ++t)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) S[t][r] *= gn;
-  bf8v kn = ck.at<row_bytes(KT)>(lk, 0, 0);
+  for (int t = 0; t < KT; ++t) kf[0][t] = ck.at<row_bytes(KT)>(lk, t, 0);
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     const float* w = pw + 16 * s;
@@ -166,32 +117,37 @@ __device__ __forceinline__ void update(f16v (&S)[KT], const bf8v (&vf)[2], const
     sldm::bf16x8 hi, mid, lo;
     if constexpr (TERMS == 3) sldm::split3_bf16x8(x, hi, mid, lo);
     else sldm::split_bf16x8(x, hi, mid);
+    phase();
+    if (s == 0)
+#pragma unroll
+      for (int t = 0; t < KT; ++t) kf[1][t] = ck.at<row_bytes(KT)>(lk, t, 1);
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
-      const bf8v kf = kn;
-      if (s * KT + t + 1 < 2 * KT) kn = ck.at<row_bytes(KT)>(lk, (t + 1) % KT, s + (t + 1) / KT);
-      if constexpr (TERMS == 3) S[t] = mfma(kf, as_bf8(lo), S[t]);
-      S[t] = mfma(kf, as_bf8(mid), S[t]);
-      S[t] = mfma(kf, as_bf8(hi), S[t]);
-      phase();
+      if (s == 0)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[t][r] *= gn;
+      if constexpr (TERMS == 3) S[t] = mfma(kf[s][t], as_bf8(lo), S[t]);
+      S[t] = mfma(kf[s][t], as_bf8(mid), S[t]);
+      S[t] = mfma(kf[s][t], as_bf8(hi), S[t]);
     }
+    phase();
   }
 }
 
 // OUT: outputs, else the state alone.  EXACT: the roundings of a short sequence or
-// an output state (above).  FAST: by Tile, else by tile_slow.
+// an output state (above).  FAST: by DMA, else by Tile::slow.
 template <int KT, int NW, bool OUT, bool EXACT, bool FAST>
 __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_bf16_kernel(Args a) {
-  using TK = Tile<KT, NW>;
-  using TV = Tile<NW, NW>;
-  constexpr int NTH = 64 * NW, RBK = TK::RB, RBV = TV::RB;
+  using TK = Tile<uint16_t, C, row_bytes(KT), NW, Swizzle>;
+  using TV = Tile<uint16_t, C, row_bytes(NW), NW, Swizzle>;
+  constexpr int NTH = 64 * NW, RBK = TK::kRB, RBV = TV::kRB;
   constexpr int kBuf = TK::BYTES * (OUT ? 2 : 1) + TV::BYTES;       // k, v, q
   __shared__ __attribute__((aligned(1024))) char tiles[2 * kBuf];
   __shared__ __attribute__((aligned(16))) float wtab[C], dtab[2 * C];
 
-  const int id = xcd_order();
+  const int order = xcd_order(), id = order / a.roles;
   if (id >= a.groups) return;
-  const Role& R = a.role[blockIdx.y];
+  const Role& R = a.role[order % a.roles];
   const Span sp = span_of(a, R, id);
   const int seg = (int)(sp.seg0 / a.seg_len);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -211,18 +167,18 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_bf16_kernel(Ar
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_vptr)tiles;
   auto fetch = [&](int64_t c, int first) {
     const uint32_t at = lds0 + (uint32_t)(c & 1) * kBuf;
-    tk.load(c, at, first, wave, lane);
-    tv.load(c, at + TK::BYTES, first, wave, lane);
-    if constexpr (OUT) tq.load(c, at + TK::BYTES + TV::BYTES, first, wave, lane);
+    tk.load(c, at, first);
+    tv.load(c, at + TK::BYTES, first);
+    if constexpr (OUT) tq.load(c, at + TK::BYTES + TV::BYTES, first);
   };
   if (FAST && nch > 0) {
     if (pad > 0 || kd < 32 * KT || vd < 32 * NW) {
       for (int i = threadIdx.x; i < 2 * kBuf / 16; i += NTH) reinterpret_cast<uint4*>(tiles)[i] = make_uint4(0, 0, 0, 0);
       __syncthreads();
     }
-    tk.init(R.k, kh, sp, sign, pad, kd, wave, lane);
-    tv.init(R.v, vh, sp, sign, pad, vd, wave, lane);
-    if constexpr (OUT) tq.init(R.q, qh, sp, sign, pad, kd, wave, lane);
+    tk.init(R.k, kh, sp, sign, pad, kd);
+    tv.init(R.v, vh, sp, sign, pad, vd);
+    if constexpr (OUT) tq.init(R.q, qh, sp, sign, pad, kd);
     fetch(0, pad);
   }
   // state: lane = value column, register 8 s + e of tile t = row 32 t + 16 s + 8 h + e
@@ -302,9 +258,9 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_bf16_kernel(Ar
       __syncthreads();
       const int64_t x0 = c * C - pad;
       char* at = tiles + (c & 1) * kBuf;
-      tile_slow<KT, NTH>(at, kh + sp.base * R.k.st, sign * R.k.st, x0, kd);
-      tile_slow<NW, NTH>(at + TK::BYTES, vh + sp.base * R.v.st, sign * R.v.st, x0, vd);
-      if constexpr (OUT) tile_slow<KT, NTH>(at + TK::BYTES + TV::BYTES, qh + sp.base * R.q.st, sign * R.q.st, x0, kd);
+      TK::slow(at, kh + sp.base * R.k.st, sign * R.k.st, x0, kd);
+      TV::slow(at + TK::BYTES, vh + sp.base * R.v.st, sign * R.v.st, x0, vd);
+      if constexpr (OUT) TK::slow(at + TK::BYTES + TV::BYTES, qh + sp.base * R.q.st, sign * R.q.st, x0, kd);
       __syncthreads();
     }
     // the tables are read, and the operands' places worked out, anew: not kept in registers
@@ -320,13 +276,19 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_bf16_kernel(Ar
       f16v P;
 #pragma unroll
       for (int r = 0; r < 16; ++r) O[r] = P[r] = 0.f;
-      bf8v qn = rq.at(lq, 0), kn = rk.at(lk, 0);
+      constexpr int A = 2 * KT < 3 ? 2 * KT : 3;                // operands in flight
+      bf8v qn[A], kn[A];
+#pragma unroll
+      for (int t = 0; t < A; ++t) {
+        qn[t] = rq.at(lq, t);
+        kn[t] = rk.at(lk, t);
+      }
 #pragma unroll
       for (int t = 0; t < 2 * KT; ++t) {
-        const bf8v qf = qn, kf = kn;
-        if (t + 1 < 2 * KT) {
-          qn = rq.at(lq, t + 1);
-          kn = rk.at(lk, t + 1);
+        const bf8v qf = qn[t % A], kf = kn[t % A];
+        if (t + A < 2 * KT) {
+          qn[t % A] = rq.at(lq, t + A);
+          kn[t % A] = rk.at(lk, t + A);
         }
         float x[8];
 #pragma unroll
@@ -380,36 +342,23 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_bf16_kernel(Ar
 }
 
 template <int KT, int NW, bool OUT, bool EXACT, bool FAST = true>
-void launch(const Args& a, int roles, hipStream_t st) {
+void launch(const Args& a, hipStream_t st) {
   decay_bf16_kernel<KT, NW, OUT, EXACT, FAST>
-      <<<dim3((unsigned)((a.groups + 7) / 8 * 8), roles), 64 * NW, 0, st>>>(a);
+      <<<grid_of(a), 64 * NW, 0, st>>>(a);
 }
 template <int KT, bool OUT, bool EXACT>
-void by_cols(const Args& a, int nw, int roles, hipStream_t st) {
-  if (nw == 1) launch<KT, 1, OUT, EXACT>(a, roles, st);
-  else if (nw == 2) launch<KT, 2, OUT, EXACT>(a, roles, st);
-  else launch<KT, 4, OUT, EXACT>(a, roles, st);
+void by_cols(const Args& a, int nw, hipStream_t st) {
+  if (nw == 1) launch<KT, 1, OUT, EXACT>(a, st);
+  else if (nw == 2) launch<KT, 2, OUT, EXACT>(a, st);
+  else launch<KT, 4, OUT, EXACT>(a, st);
 }
 template <bool OUT, bool EXACT>
-void by_rows(const Args& a, int roles, hipStream_t st) {
+void by_rows(const Args& a, hipStream_t st) {
   const int kt = row_tiles(a.role[0].kd), nw = tiles_of(a.role[0].vd);
-  if (kt == 1) by_cols<1, OUT, EXACT>(a, nw, roles, st);
-  else if (kt == 2) by_cols<2, OUT, EXACT>(a, nw, roles, st);
-  else if (kt == 3) by_cols<3, OUT, EXACT>(a, nw, roles, st);
-  else by_cols<4, OUT, EXACT>(a, nw, roles, st);
+  if (kt == 1) by_cols<1, OUT, EXACT>(a, nw, st);
+  else if (kt == 2) by_cols<2, OUT, EXACT>(a, nw, st);
+  else if (kt == 3) by_cols<3, OUT, EXACT>(a, nw, st);
+  else by_cols<4, OUT, EXACT>(a, nw, st);
 }
-// Rows of a chunk within 32-bit byte offsets of each other.
-inline bool near(const Operand& t) { return t.st >= 0 && t.st < ((int64_t)1 << 25); }
-// Every operand's rows on 16-byte boundaries and whole granules.
-inline bool all_fast(const Args& a, int roles, bool out) {
-  bool ok = true;
-  for (int i = 0; i < roles; ++i) {
-    const Role& r = a.role[i];
-    ok = ok && r.k.vec && r.v.vec && r.kd % 8 == 0 && r.vd % 8 == 0 && (!out || (r.q.vec && r.o_vec)) &&
-         near(r.k) && near(r.v) && (!out || near(r.q));
-  }
-  return ok;
-}
-
 }  // namespace
 }  // namespace sldm_decay

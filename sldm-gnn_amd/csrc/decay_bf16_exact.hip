@@ -3,5 +3,5 @@
 #include "decay_bf16.hpp"
 
 namespace sldm_decay {
-void run_bf16_exact(const Args& a, int roles, hipStream_t st) { by_rows<true, true>(a, roles, st); }
+void run_bf16_exact(const Args& a, hipStream_t st) { by_rows<true, true>(a, st); }
 }  // namespace sldm_decay

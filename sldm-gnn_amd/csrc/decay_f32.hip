@@ -1,15 +1,16 @@
 // Decay attention in fp32 (mathematics: decay.hpp): chunks of 16 tokens on
-// v_mfma_f32_16x16x4_f32, operands straight from memory.
+// v_mfma_f32_16x16x4_f32.
 //
-// A wave owns 16 or 32 value columns of one (batch, head, segment) and nothing
-// is shared: no LDS, no barrier.  In fp32 an operand is one value a lane and
-// product, so rows come as 16 bytes a lane (q, k: lane = row, four neighbouring
-// columns are four products' contraction slots), and the transposed operands of
-// P V and K^T V (lane = column) as 4-byte loads whose 16 lanes share a 64-byte
-// piece of a row.  The chunk is as short as a tile because the products inside a
-// chunk cost C (Dk + Dv) a token against 2 Dk Dv between chunks, and because a
-// 16-wide head then wastes no part of a tile.  The next chunk's q and k are
-// loaded over this chunk's second half, k^T and v over its first.
+// A workgroup owns one (batch, head, segment), a wave 16 or 32 value columns and
+// their slice of the state, in accumulators for the whole walk.  Tiles of SUB
+// chunks of q, k and v come by LDS-DMA into two buffers, the next tile's while
+// this one is computed, with one barrier a tile.  An fp32 operand is one value a
+// lane and product, so rows are read 16 bytes a lane (lane = row: four
+// neighbouring columns are four products' contraction slots) and columns 4 bytes
+// a lane.  The chunk is as short as the matrix tile: the products inside a chunk
+// cost C (Dk + Dv) a token against 2 Dk Dv between chunks, and a 16-wide head
+// wastes no part of a tile.  Bound by the fp32 matrix rate from 64-wide heads on,
+// by memory below.
 #include "decay.hpp"
 
 namespace sldm_decay {
@@ -21,32 +22,72 @@ constexpr int C = 16;
 __device__ __forceinline__ f4v mfma(float a, float b, f4v c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
-// four columns from `col` of a row of d; zeros past d
-__device__ __forceinline__ f4v load4(const float* row, int col, int d, bool vec) {
-  if (vec) return col < d ? *reinterpret_cast<const f4v*>(row + col) : f4v{0.f, 0.f, 0.f, 0.f};
-  f4v v;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = col + e < d ? row[col + e] : 0.f;
-  return v;
-}
 
-template <int KT, int NV, bool OUT>
-__global__ __launch_bounds__(256) void decay_f32_kernel(Args a) {
-  const Role& R = a.role[blockIdx.y];
-  const int slices = (R.vd + 16 * NV - 1) / (16 * NV);
-  const int task = xcd_order() * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int id = task / slices, v0 = task % slices * 16 * NV;
+// Granule g of row r lies at g ^ swz(r): a column read's rows 4 h + r (64 bytes of
+// each) fall into different quarters of the banks where a row has four, the 16
+// rows of a row read into 16 places.
+template <int RB>
+struct Swizzle {
+  static __device__ __forceinline__ int of(int r) {
+    return RB == 64 ? (r >> 2) & 3 : RB == 128 ? (r & 4) | ((r >> 1) & 1) | ((r >> 2) & 2) : (r & 12) | (r & 3);
+  }
+};
+
+// KT: tiles of 16 state rows; NV: of 16 value columns a wave.  OUT: outputs, else
+// the state alone.  FAST: by DMA, else by Tile::slow.
+template <int KT, int NV, int NW, int SUB, bool OUT, bool FAST>
+__global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_f32_kernel(Args a) {
+  constexpr int RBK = KT == 6 ? 512 : 64 * KT, RBV = 64 * NV * NW, ROWS = C * SUB, NTH = 64 * NW;
+  using TK = Tile<float, ROWS, RBK, NW, Swizzle>;
+  using TV = Tile<float, ROWS, RBV, NW, Swizzle>;
+  constexpr int kBuf = TK::BYTES * (OUT ? 2 : 1) + TV::BYTES;       // k, v, q
+  __shared__ __attribute__((aligned(1024))) char tiles[2 * kBuf];
+
+  const int order = xcd_order(), id = order / a.roles;
   if (id >= a.groups) return;
-  const Span s = span_of(a, R, id);
+  const Role& R = a.role[order % a.roles];
+  const Span sp = span_of(a, R, id);
+  const int seg = (int)(sp.seg0 / a.seg_len);
   const int lane = threadIdx.x & 63, m = lane & 15, h = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), v0 = 16 * NV * wave;
   const int kd = R.kd, vd = R.vd;
-  const float ld2 = a.log_decay[s.hd] * 1.44269504088896340736f;
-  const int seg = (int)(s.seg0 / a.seg_len);
+  const int pad = (int)((ROWS - sp.n % ROWS) % ROWS);
+  const int64_t nt = (sp.n + pad) / ROWS;
+  const int64_t sign = R.reverse ? -1 : 1;
+  const float ld2 = a.log_decay[sp.hd] * 1.44269504088896340736f;
+
+  const float* qh = OUT ? reinterpret_cast<const float*>(R.q.p) + sp.b * R.q.sb + (sp.hd / R.q.hdiv) * R.q.sh : nullptr;
+  const float* kh = reinterpret_cast<const float*>(R.k.p) + sp.b * R.k.sb + (sp.hd / R.k.hdiv) * R.k.sh;
+  const float* vh = reinterpret_cast<const float*>(R.v.p) + sp.b * R.v.sb + (sp.hd / R.v.hdiv) * R.v.sh;
+
+  TK tq, tk;
+  TV tv;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_vptr)tiles;
+  auto fetch = [&](int64_t c, int first) {
+    const uint32_t at = lds0 + (uint32_t)(c & 1) * kBuf;
+    tk.load(c, at, first);
+    tv.load(c, at + TK::BYTES, first);
+    if constexpr (OUT) tq.load(c, at + TK::BYTES + TV::BYTES, first);
+  };
+  if (FAST && nt > 0) {
+    if (pad > 0 || kd * 4 < RBK || vd * 4 < RBV) {
+      for (int i = threadIdx.x; i < 2 * kBuf / 16; i += NTH) reinterpret_cast<uint4*>(tiles)[i] = make_uint4(0, 0, 0, 0);
+      __syncthreads();
+    }
+    tk.init(R.k, kh, sp, sign, pad, kd);
+    tv.init(R.v, vh, sp, sign, pad, vd);
+    if constexpr (OUT) tq.init(R.q, qh, sp, sign, pad, kd);
+    fetch(0, pad);
+  }
 
   // state: lane = value column, registers = state rows 16 t + 4 h + r
   f4v S[KT][NV];
-  {
-    const float* s0 = R.s0 ? R.s0 + s.bh * R.s0_bh + seg * R.s0_seg : nullptr;
+#pragma unroll
+  for (int t = 0; t < KT; ++t)
+#pragma unroll
+    for (int v = 0; v < NV; ++v) S[t][v] = f4v{0.f, 0.f, 0.f, 0.f};
+  if (R.s0) {
+    const float* s0 = R.s0 + sp.bh * R.s0_bh + seg * R.s0_seg;
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -54,47 +95,9 @@ __global__ __launch_bounds__(256) void decay_f32_kernel(Args a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int kr = 16 * t + 4 * h + r, vc = v0 + 16 * v + m;
-          S[t][v][r] = s0 && kr < kd && vc < vd ? s0[kr * R.s_k + vc * R.s_v] : 0.f;
+          if (kr < kd && vc < vd) S[t][v][r] = s0[kr * R.s_k + vc * R.s_v];
         }
   }
-
-  const int pad = (int)((C - s.n % C) % C);
-  const int64_t nch = (s.n + pad) / C;
-  const int64_t sign = R.reverse ? -1 : 1;
-  const bool qvec = R.q.vec && kd % 4 == 0, kvec = R.k.vec && kd % 4 == 0;
-  const float* qh = reinterpret_cast<const float*>(R.q.p) + s.b * R.q.sb + (s.hd / R.q.hdiv) * R.q.sh;
-  const float* kh = reinterpret_cast<const float*>(R.k.p) + s.b * R.k.sb + (s.hd / R.k.hdiv) * R.k.sh;
-  const float* vh = reinterpret_cast<const float*>(R.v.p) + s.b * R.v.sb + (s.hd / R.v.hdiv) * R.v.sh;
-  const int64_t q_row = sign * m * R.q.st, k_row = sign * m * R.k.st;
-
-  f4v q[KT], k[KT], kt[KT], vv[NV];
-  auto load_rows = [&](int64_t x0, bool first) {     // q, k: lane = row m
-    const int64_t tok = s.base + sign * x0;
-    const float *qp = qh + tok * R.q.st + q_row, *kp = kh + tok * R.k.st + k_row;
-    const bool on = !first || x0 + m >= 0;
-#pragma unroll
-    for (int t = 0; t < KT; ++t) {
-      q[t] = k[t] = f4v{0.f, 0.f, 0.f, 0.f};
-      if (on && 16 * t < kd) {
-        q[t] = load4(qp, 16 * t + 4 * h, kd, qvec);
-        k[t] = load4(kp, 16 * t + 4 * h, kd, kvec);
-      }
-    }
-  };
-  auto load_cols = [&](int64_t x0, bool first) {     // k^T, v: lane = column, registers = rows 4 h + r
-    const int64_t tok = s.base + sign * x0;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int j = 4 * h + r;
-      const bool on = !first || x0 + j >= 0;
-      const float *kp = kh + tok * R.k.st + sign * j * R.k.st, *vp = vh + tok * R.v.st + sign * j * R.v.st;
-#pragma unroll
-      for (int t = 0; t < KT; ++t) kt[t][r] = on && 16 * t + m < kd ? kp[16 * t + m] : 0.f;
-#pragma unroll
-      for (int v = 0; v < NV; ++v) vv[v][r] = on && v0 + 16 * v + m < vd ? vp[v0 + 16 * v + m] : 0.f;
-    }
-  };
-
   float d[4], w[4];                                  // D (lane = i, registers = j), the update's weights
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
@@ -102,76 +105,125 @@ __global__ __launch_bounds__(256) void decay_f32_kernel(Args a) {
     d[r] = m >= j ? powg(ld2, m - j) * R.p_scale : 0.f;
     w[r] = powg(ld2, C - 1 - j + R.delta) * R.upd_scale;
   }
-  bool have_state = R.s0 != nullptr;
-  if (OUT && nch > 0) load_rows(-pad, true);
-  for (int64_t c = 0; c < nch; ++c) {
-    const int64_t x0 = c * C - pad;
-    const int padc = c == 0 ? pad : 0;
-    load_cols(x0, c == 0);
-    f4v O[NV];
-    f4v P = {0.f, 0.f, 0.f, 0.f};
-    if constexpr (OUT) {
+  const float rd_full = powg(ld2, m + 1 - R.delta) * R.read_scale, gn_full = powg(ld2, C);
+
+  // where a lane finds granule h of row m, and column m of row 4 h; the swizzles are
+  // XORs of bits, so other tiles and rows flip constant bits of the places
+  const int row_at = m * RBK, kcol_at = 4 * h * RBK + 4 * (m & 3), vcol_at = 4 * h * RBV + 4 * (m & 3);
+  int row_x = (h ^ Swizzle<RBK>::of(m)) << 4, kcol_x = (m >> 2 ^ Swizzle<RBK>::of(4 * h)) << 4;
+  const int vcol_x = (m >> 2 ^ Swizzle<RBV>::of(4 * h)) << 4;
+  f4v O[SUB][NV];
+  auto put = [&](int64_t c) {
 #pragma unroll
-      for (int v = 0; v < NV; ++v) O[v] = f4v{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int t = 0; t < KT; ++t)
-        if (16 * t < kd)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) P = mfma(k[t][r], q[t][r], P);
-      if (have_state) {
-#pragma unroll
-        for (int t = 0; t < KT; ++t)
-          if (16 * t < kd)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-              for (int v = 0; v < NV; ++v) O[v] = mfma(S[t][v][r], q[t][r], O[v]);
-        const float rd = powg(ld2, m - padc + 1 - R.delta) * R.read_scale;
-#pragma unroll
-        for (int v = 0; v < NV; ++v) O[v] *= rd;
-      }
-      if (c + 1 < nch) load_rows(x0 + C, false);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float p = P[r] * d[r];
-#pragma unroll
-        for (int v = 0; v < NV; ++v) O[v] = mfma(vv[v][r], p, O[v]);
-      }
-    }
-    const float gn = powg(ld2, C - padc);
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int v = 0; v < NV; ++v) S[t][v] *= gn;
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int s = 0; s < SUB; ++s) {
+      const int64_t x = c * ROWS + C * s + m - pad;
+      if (x < 0) continue;
+      float* o = reinterpret_cast<float*>(R.o) + sp.b * R.o_sb + (sp.base + sign * x) * R.o_st + sp.hd * R.o_sh;
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        const float u = vv[v][r] * w[r];
+        const int c0 = v0 + 16 * v + 4 * h;
+        if (FAST) {
+          if (c0 < vd) *reinterpret_cast<f4v*>(o + c0) = O[s][v];
+        } else {
 #pragma unroll
-        for (int t = 0; t < KT; ++t)
-          if (16 * t < kd) S[t][v] = mfma(kt[t][r], u, S[t][v]);
-      }
-    have_state = true;
-    if constexpr (OUT) {
-      if (x0 + m >= 0) {
-        float* o = reinterpret_cast<float*>(R.o) + s.b * R.o_sb + (s.base + sign * (x0 + m)) * R.o_st + s.hd * R.o_sh;
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-          const int c0 = v0 + 16 * v + 4 * h;
-          if (R.o_vec) {
-            if (c0 < vd) *reinterpret_cast<f4v*>(o + c0) = O[v];
-          } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (c0 + r < vd) o[c0 + r] = O[v][r];
-          }
+          for (int r = 0; r < 4; ++r)
+            if (c0 + r < vd) o[c0 + r] = O[s][v][r];
         }
       }
     }
+  };
+
+  for (int64_t c = 0; c < nt; ++c) {
+    if constexpr (FAST) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // this tile (and older stores)
+      __syncthreads();                                          // of all waves; the other buffer is free
+      if (OUT && c > 0) put(c - 1);
+      if (c + 1 < nt) fetch(c + 1, 0);
+    } else {
+      if (OUT && c > 0) put(c - 1);
+      __syncthreads();
+      const int64_t x0 = c * ROWS - pad;
+      char* at = tiles + (c & 1) * kBuf;
+      TK::slow(at, kh + sp.base * R.k.st, sign * R.k.st, x0, kd);
+      TV::slow(at + TK::BYTES, vh + sp.base * R.v.st, sign * R.v.st, x0, vd);
+      if constexpr (OUT) TK::slow(at + TK::BYTES + TV::BYTES, qh + sp.base * R.q.st, sign * R.q.st, x0, kd);
+      __syncthreads();
+    }
+    asm volatile("" : "+v"(row_x), "+v"(kcol_x) :: "memory");   // operands' places are worked out anew, not kept
+#pragma unroll
+    for (int s = 0; s < SUB; ++s) {
+      const int empty = c == 0 ? pad - C * s : 0;               // rows in front of the segment
+      if (SUB > 1 && empty >= C) continue;
+      const char* lk = tiles + (c & 1) * kBuf + C * s * RBK;
+      const char* lv = tiles + (c & 1) * kBuf + TK::BYTES + C * s * RBV;
+      const char* lq = tiles + (c & 1) * kBuf + TK::BYTES + TV::BYTES + C * s * RBK;
+      const int padc = empty > 0 ? empty : 0;
+      f4v vv[NV];
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          vv[v][r] = *reinterpret_cast<const float*>(
+              lv + vcol_at + r * RBV + (vcol_x ^ (64 * (NV * wave + v)) ^ (Swizzle<RBV>::of(r) << 4)));
+      auto kcol = [&](int t) {
+        f4v x;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          x[r] = *reinterpret_cast<const float*>(
+              lk + kcol_at + r * RBK + (kcol_x ^ (64 * t) ^ (Swizzle<RBK>::of(r) << 4)));
+        return x;
+      };
+      if constexpr (OUT) {
+        f4v P = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int v = 0; v < NV; ++v) O[s][v] = f4v{0.f, 0.f, 0.f, 0.f};
+        f4v qn = *reinterpret_cast<const f4v*>(lq + row_at + row_x), kn = *reinterpret_cast<const f4v*>(lk + row_at + row_x);
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          const f4v q = qn, k = kn;
+          if (t + 1 < KT) {
+            qn = *reinterpret_cast<const f4v*>(lq + row_at + (row_x ^ 64 * (t + 1)));
+            kn = *reinterpret_cast<const f4v*>(lk + row_at + (row_x ^ 64 * (t + 1)));
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            P = mfma(k[r], q[r], P);
+#pragma unroll
+            for (int v = 0; v < NV; ++v) O[s][v] = mfma(S[t][v][r], q[r], O[s][v]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        const float rd = padc ? powg(ld2, m - padc + 1 - R.delta) * R.read_scale : rd_full;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) O[s][v] *= rd;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int v = 0; v < NV; ++v) O[s][v] = mfma(vv[v][r], P[r] * d[r], O[s][v]);
+      }
+      const float gn = padc ? powg(ld2, C - padc) : gn_full;
+      f4v kn = kcol(0);
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) vv[v][r] *= w[r];
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        const f4v k = kn;
+        if (t + 1 < KT) kn = kcol(t + 1);
+#pragma unroll
+        for (int v = 0; v < NV; ++v) S[t][v] *= gn;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int v = 0; v < NV; ++v) S[t][v] = mfma(k[r], vv[v][r], S[t][v]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
   }
+  if (OUT && nt > 0) put(nt - 1);
   if (R.s1) {
-    float* s1 = R.s1 + s.bh * R.s1_bh + seg * R.s1_seg;
+    float* s1 = R.s1 + sp.bh * R.s1_bh + seg * R.s1_seg;
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -182,44 +234,47 @@ __global__ __launch_bounds__(256) void decay_f32_kernel(Args a) {
           if (kr < kd && vc < vd) s1[kr * R.s_k + vc * R.s_v] = S[t][v][r];
         }
   }
-  if constexpr (OUT) {                               // tokens behind the sequence's end: zeros
-    const int64_t t1 = s.seg0 + a.seg_len < a.T ? s.seg0 + a.seg_len : a.T;
-    const int cols = vd - v0 < 16 * NV ? vd - v0 : 16 * NV;
-    for (int64_t t = s.len > s.seg0 ? s.len : s.seg0; t < t1; ++t)
-      if (lane < cols)
-        reinterpret_cast<float*>(R.o)[s.b * R.o_sb + t * R.o_st + s.hd * R.o_sh + v0 + lane] = 0.f;
+  if constexpr (OUT) {                                          // tokens behind the sequence's end: zeros
+    const int64_t t1 = sp.seg0 + a.seg_len < a.T ? sp.seg0 + a.seg_len : a.T;
+    const int64_t t0 = sp.len > sp.seg0 ? sp.len : sp.seg0;
+    const int64_t todo = t1 > t0 ? (t1 - t0) * vd : 0;
+    for (int64_t i = threadIdx.x; i < todo; i += NTH)
+      reinterpret_cast<float*>(R.o)[sp.b * R.o_sb + (t0 + i / vd) * R.o_st + sp.hd * R.o_sh + i % vd] = 0.f;
   }
 }
 
+template <int KT, int NV, int NW, int SUB, bool OUT, bool FAST = true>
+void launch(const Args& a, hipStream_t st) {
+  decay_f32_kernel<KT, NV, NW, SUB, OUT, FAST>
+      <<<grid_of(a), 64 * NW, 0, st>>>(a);
+}
+// Tiles of 32 tokens while a head is narrow, of 16 where 32 would leave a CU short
+// of workgroups.
 template <int KT, bool OUT>
-void launch(const Args& a, int roles, hipStream_t st) {
-  int vd = 0;
-  for (int i = 0; i < roles; ++i) vd = a.role[i].vd > vd ? a.role[i].vd : vd;
-  const int nv = vd <= 16 ? 1 : 2;
-  int64_t most = 0;
-  for (int i = 0; i < roles; ++i) {
-    const int64_t w = (int64_t)a.groups * ((a.role[i].vd + 16 * nv - 1) / (16 * nv));
-    most = w > most ? w : most;
-  }
-  const unsigned grid = (unsigned)((most + 31) / 32 * 8);
-  if (nv == 1) decay_f32_kernel<KT, 1, OUT><<<dim3(grid, roles), 256, 0, st>>>(a);
-  else decay_f32_kernel<KT, 2, OUT><<<dim3(grid, roles), 256, 0, st>>>(a);
+void by_cols(const Args& a, int vd, hipStream_t st) {
+  constexpr int SUB = KT <= 2 ? 2 : 1;
+  if (vd <= 16) launch<KT, 1, 1, SUB, OUT>(a, st);
+  else if (vd <= 32) launch<KT, 2, 1, SUB, OUT>(a, st);
+  else if (vd <= 64) launch<KT, 2, 2, 1, OUT>(a, st);
+  else launch<KT, 2, 4, 1, OUT>(a, st);
 }
-
 template <bool OUT>
-void by_rows(const Args& a, int roles, hipStream_t st) {
-  int kd = 0;
-  for (int i = 0; i < roles; ++i) kd = a.role[i].kd > kd ? a.role[i].kd : kd;
-  if (kd <= 16) launch<1, OUT>(a, roles, st);
-  else if (kd <= 32) launch<2, OUT>(a, roles, st);
-  else if (kd <= 64) launch<4, OUT>(a, roles, st);
-  else launch<8, OUT>(a, roles, st);
+void run(const Args& a, hipStream_t st) {
+  int kd = 0, vd = 0;
+  for (int i = 0; i < a.roles; ++i) {
+    kd = a.role[i].kd > kd ? a.role[i].kd : kd;
+    vd = a.role[i].vd > vd ? a.role[i].vd : vd;
+  }
+  if (!all_fast(a, OUT, 4)) launch<8, 2, 4, 1, OUT, false>(a, st);
+  else if (kd <= 16) by_cols<1, OUT>(a, vd, st);
+  else if (kd <= 32) by_cols<2, OUT>(a, vd, st);
+  else if (kd <= 64) by_cols<4, OUT>(a, vd, st);
+  else if (kd <= 96) by_cols<6, OUT>(a, vd, st);
+  else by_cols<8, OUT>(a, vd, st);
 }
 
 }  // namespace
 
-void run_f32(const Args& a, int roles, bool out, hipStream_t st) {
-  out ? by_rows<true>(a, roles, st) : by_rows<false>(a, roles, st);
-}
+void run_f32(const Args& a, bool out, hipStream_t st) { out ? run<true>(a, st) : run<false>(a, st); }
 
 }  // namespace sldm_decay
