@@ -46,8 +46,19 @@ __global__ __launch_bounds__(256) void scan_kernel(float* loc, const float* s0, 
   float run = s0 ? s0[bh * elems + e] : 0.f;
   float* p = loc + bh * a.nseg * elems + e;
   const float g = exp2f(ld2 * (float)a.seg_len);
+  const int whole = (int)(len / a.seg_len);   // segments without padding
   int s = 0;
-  for (; s < a.nseg && (int64_t)(s + 1) * a.seg_len <= len; ++s) {
+  for (; s + 8 <= whole; s += 8) {             // eight loads in flight
+    float add[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) add[i] = p[(s + i) * elems];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      p[(s + i) * elems] = run;
+      run = run * g + add[i];
+    }
+  }
+  for (; s < whole; ++s) {
     const float add = p[s * elems];
     p[s * elems] = run;
     run = run * g + add;
@@ -171,6 +182,9 @@ void launch_roles(int dtype, Args& a, const Role* const* roles, int n, bool out,
         done[j] = true;
       }
     a.roles = m;
+    // heads whose rows share 256 bytes
+    const int64_t row = std::max<int64_t>(1, std::min(a.role[0].kd, a.role[0].vd)) * (dtype == SLDM_F32 ? 4 : 2);
+    a.unit = m * (int)std::max<int64_t>(1, std::min<int64_t>(a.H, 256 / row));
     if (dtype == SLDM_F32) run_f32(a, out, st);
     else run_bf16(a, out, st);
   }

@@ -58,7 +58,7 @@ struct Args {
   Role role[3];
   int64_t B, H, T, seg_len;
   int nseg, groups;     // groups = B H nseg
-  int roles;
+  int roles, unit;      // unit: workgroups that stay together on an XCD
   const float* log_decay;
   const void* lengths;  // null: T each
   int lengths64;
@@ -73,11 +73,14 @@ __device__ __forceinline__ int64_t seq_len(const Args& a, int64_t b) {
   return n < 0 ? 0 : (n > a.T ? a.T : n);
 }
 
-// Workgroups are dealt to the XCDs in turn; neighbours in (segment, batch, head,
-// role) order are put on one XCD: heads share cache lines, and the roles of one
-// head read the same tensors.  gridDim.x is a multiple of 8.
-__device__ __forceinline__ int xcd_order() {
-  return ((int)blockIdx.x & 7) * ((int)gridDim.x >> 3) + ((int)blockIdx.x >> 3);
+// Workgroups are dealt to the XCDs in turn.  Units of neighbours in (segment,
+// batch, head, role) order stay on one XCD: the roles of a head read the same
+// tensors, and narrow heads share cache lines.  The units themselves go round the
+// XCDs, one place further each time, so that batches of uneven lengths do not
+// load some XCDs alone (ragged prompts: whole ranges of units an XCD 105 us).
+__device__ __forceinline__ int xcd_order(int unit) {
+  const int slot = (int)blockIdx.x >> 3, turn = slot / unit;
+  return (turn * 8 + (((int)blockIdx.x + turn) & 7)) * unit + slot % unit;
 }
 
 // What a (batch, head, segment) is made of.
@@ -154,6 +157,26 @@ struct Tile {
   }
 };
 
+// Tokens behind the sequence's end (of this segment's range): zeros, 16 bytes a
+// thread where the rows allow it.
+template <int NTH, bool FAST>
+__device__ __forceinline__ void zero_tail(const Args& a, const Role& R, const Span& s, int elem_bytes) {
+  const int64_t t1 = s.seg0 + a.seg_len < a.T ? s.seg0 + a.seg_len : a.T;
+  const int64_t t0 = s.len > s.seg0 ? s.len : s.seg0;
+  if (t0 >= t1) return;
+  constexpr int kLanes = 32;                     // across a row (of at most 512 bytes: 32 granules)
+  const int col = (int)threadIdx.x % kLanes, bytes = R.vd * elem_bytes;
+  char* o = reinterpret_cast<char*>(R.o) + (s.b * R.o_sb + s.hd * R.o_sh) * elem_bytes;
+  for (int64_t t = t0 + (int)threadIdx.x / kLanes; t < t1; t += NTH / kLanes) {
+    char* row = o + t * R.o_st * elem_bytes;
+    if (FAST) {
+      if (16 * col < bytes) *reinterpret_cast<uint4*>(row + 16 * col) = make_uint4(0, 0, 0, 0);
+    } else {
+      for (int i = 2 * col; i < bytes; i += 2 * kLanes) *reinterpret_cast<uint16_t*>(row + i) = 0;
+    }
+  }
+}
+
 // Rows of a chunk within 32-bit byte offsets of each other.
 inline bool near(const Operand& t) { return t.st >= 0 && t.st < ((int64_t)1 << 24); }
 // Whether every operand can come by DMA: rows on 16-byte boundaries, whole granules.
@@ -171,7 +194,10 @@ inline bool all_fast(const Args& a, bool out, int granule) {
 // out: roles write outputs; else states only.
 void run_bf16(const Args& a, bool out, hipStream_t stream);
 void run_f32(const Args& a, bool out, hipStream_t stream);
-inline unsigned grid_of(const Args& a) { return (unsigned)(((int64_t)a.groups * a.roles + 7) / 8 * 8); }
+inline unsigned grid_of(const Args& a) {
+  const int64_t n = (int64_t)a.groups * a.roles, u = 8 * a.unit;
+  return (unsigned)((n + u - 1) / u * u);
+}
 inline int tiles_of(int d) { return d <= 32 ? 1 : d <= 64 ? 2 : 4; }   // waves across vd
 inline int row_tiles(int d) { return (d + 31) / 32; }
 

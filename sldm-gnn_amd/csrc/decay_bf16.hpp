@@ -145,7 +145,7 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_bf16_kernel(Ar
   __shared__ __attribute__((aligned(1024))) char tiles[2 * kBuf];
   __shared__ __attribute__((aligned(16))) float wtab[C], dtab[2 * C];
 
-  const int order = xcd_order(), id = order / a.roles;
+  const int order = xcd_order(a.unit), id = order / a.roles;
   if (id >= a.groups) return;
   const Role& R = a.role[order % a.roles];
   const Span sp = span_of(a, R, id);
@@ -329,16 +329,7 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_bf16_kernel(Ar
         if (kr < kd && vc < vd) s1[kr * R.s_k + vc * R.s_v] = S[t][r];
       }
   }
-  if constexpr (OUT) {                                          // tokens behind the sequence's end: zeros
-    const int64_t t1 = sp.seg0 + a.seg_len < a.T ? sp.seg0 + a.seg_len : a.T;
-    const int64_t t0 = sp.len > sp.seg0 ? sp.len : sp.seg0;
-    const int64_t todo = t1 > t0 ? (t1 - t0) * vd : 0;
-    for (int64_t i = threadIdx.x; i < todo; i += NTH) {
-      const int64_t off = sp.b * R.o_sb + (t0 + i / vd) * R.o_st + sp.hd * R.o_sh + i % vd;
-      if (R.o_f32) reinterpret_cast<float*>(R.o)[off] = 0.f;
-      else reinterpret_cast<uint16_t*>(R.o)[off] = 0;
-    }
-  }
+  if constexpr (OUT) zero_tail<NTH, FAST>(a, R, sp, R.o_f32 ? 4 : 2);
 }
 
 template <int KT, int NW, bool OUT, bool EXACT, bool FAST = true>

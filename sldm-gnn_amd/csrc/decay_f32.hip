@@ -43,7 +43,7 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_f32_kernel(Arg
   constexpr int kBuf = TK::BYTES * (OUT ? 2 : 1) + TV::BYTES;       // k, v, q
   __shared__ __attribute__((aligned(1024))) char tiles[2 * kBuf];
 
-  const int order = xcd_order(), id = order / a.roles;
+  const int order = xcd_order(a.unit), id = order / a.roles;
   if (id >= a.groups) return;
   const Role& R = a.role[order % a.roles];
   const Span sp = span_of(a, R, id);
@@ -234,13 +234,7 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_f32_kernel(Arg
           if (kr < kd && vc < vd) s1[kr * R.s_k + vc * R.s_v] = S[t][v][r];
         }
   }
-  if constexpr (OUT) {                                          // tokens behind the sequence's end: zeros
-    const int64_t t1 = sp.seg0 + a.seg_len < a.T ? sp.seg0 + a.seg_len : a.T;
-    const int64_t t0 = sp.len > sp.seg0 ? sp.len : sp.seg0;
-    const int64_t todo = t1 > t0 ? (t1 - t0) * vd : 0;
-    for (int64_t i = threadIdx.x; i < todo; i += NTH)
-      reinterpret_cast<float*>(R.o)[sp.b * R.o_sb + (t0 + i / vd) * R.o_st + sp.hd * R.o_sh + i % vd] = 0.f;
-  }
+  if constexpr (OUT) zero_tail<NTH, FAST>(a, R, sp, 4);
 }
 
 template <int KT, int NV, int NW, int SUB, bool OUT, bool FAST = true>
