@@ -26,35 +26,58 @@ constexpr int kBlock = 256;
 typedef uint32_t u4a2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u4a4 __attribute__((ext_vector_type(4), aligned(4)));
 
-// V elements at element alignment (16-byte accesses for V = 16 / sizeof(T))
+// V elements of a row as they lie in memory, at element alignment (16-byte
+// accesses for V = 16 / sizeof(T)).
 template <typename T, int V>
-__device__ __forceinline__ void load_row(const T* p, float (&r)[V]) {
-  if constexpr (sizeof(T) * V == 16) {
-    uint4 w;
-    if constexpr (sizeof(T) == 2) w = __builtin_bit_cast(uint4, *reinterpret_cast<const u4a2*>(p));
+struct Raw {
+  static constexpr bool kWide = sizeof(T) * V == 16;
+  uint4 w;
+  T one;
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (!kWide) one = *p;
+    else if constexpr (sizeof(T) == 2) w = __builtin_bit_cast(uint4, *reinterpret_cast<const u4a2*>(p));
     else w = __builtin_bit_cast(uint4, *reinterpret_cast<const u4a4*>(p));
-    if constexpr (sizeof(T) == 2) {
+  }
+  __device__ __forceinline__ void get(float (&r)[V]) const {
+    if constexpr (!kWide) {
+      sldm::Vec<T, 1>::load(&one, r);
+    } else if constexpr (sizeof(T) == 2) {
       r[0] = sldm::bf16_lo(w.x); r[1] = sldm::bf16_hi(w.x); r[2] = sldm::bf16_lo(w.y); r[3] = sldm::bf16_hi(w.y);
       r[4] = sldm::bf16_lo(w.z); r[5] = sldm::bf16_hi(w.z); r[6] = sldm::bf16_lo(w.w); r[7] = sldm::bf16_hi(w.w);
     } else {
       r[0] = __uint_as_float(w.x); r[1] = __uint_as_float(w.y);
       r[2] = __uint_as_float(w.z); r[3] = __uint_as_float(w.w);
     }
-  } else {
-    sldm::Vec<T, V>::load(p, r);
   }
-}
+};
 template <typename T, int V>
 __device__ __forceinline__ void store_row(T* p, const float (&r)[V]) {
-  if constexpr (sizeof(T) * V == 16) {
-    if constexpr (sizeof(T) == 2)
-      *reinterpret_cast<u4a2*>(p) = u4a2{sldm::pack_bf16x2(r[0], r[1]), sldm::pack_bf16x2(r[2], r[3]),
-                                         sldm::pack_bf16x2(r[4], r[5]), sldm::pack_bf16x2(r[6], r[7])};
-    else
-      *reinterpret_cast<u4a4*>(p) = u4a4{__float_as_uint(r[0]), __float_as_uint(r[1]), __float_as_uint(r[2]),
-                                         __float_as_uint(r[3])};
-  } else {
+  if constexpr (!Raw<T, V>::kWide)
     sldm::Vec<T, V>::store(p, r);
+  else if constexpr (sizeof(T) == 2)
+    *reinterpret_cast<u4a2*>(p) = u4a2{sldm::pack_bf16x2(r[0], r[1]), sldm::pack_bf16x2(r[2], r[3]),
+                                       sldm::pack_bf16x2(r[4], r[5]), sldm::pack_bf16x2(r[6], r[7])};
+  else
+    *reinterpret_cast<u4a4*>(p) = u4a4{__float_as_uint(r[0]), __float_as_uint(r[1]), __float_as_uint(r[2]),
+                                       __float_as_uint(r[3])};
+}
+
+// V columns of weight or bias; `none` where there is none
+template <int V>
+__device__ __forceinline__ void load_param(const float* p, int f, bool on, float none, float (&r)[V]) {
+#pragma unroll
+  for (int k = 0; k < V; ++k) r[k] = none;
+  if (!p || !on) return;
+  if constexpr (V % 4 == 0) {
+#pragma unroll
+    for (int k = 0; k < V; k += 4) {
+      const u4a4 u = *reinterpret_cast<const u4a4*>(p + f + k);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[k + e] = __uint_as_float(u[e]);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) r[k] = p[f + k];
   }
 }
 
@@ -68,6 +91,23 @@ __device__ __forceinline__ float row_sum(float v, int lpr, float* red, int slot)
   if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = v;
   __syncthreads();
   return (r[0] + r[1]) + (r[2] + r[3]);
+}
+
+// Two such sums, one barrier.
+template <bool WIDE>
+__device__ __forceinline__ void row_sum2(float& u, float& v, int lpr, float* red, int slot) {
+  u = sldm::group_sum(u, WIDE ? 64 : lpr);
+  v = sldm::group_sum(v, WIDE ? 64 : lpr);
+  if constexpr (WIDE) {
+    float* r = red + slot * (2 * kBlock / 64);
+    if ((threadIdx.x & 63) == 0) {
+      r[threadIdx.x >> 6] = u;
+      r[4 + (threadIdx.x >> 6)] = v;
+    }
+    __syncthreads();
+    u = (r[0] + r[1]) + (r[2] + r[3]);
+    v = (r[4] + r[5]) + (r[6] + r[7]);
+  }
 }
 
 struct Lanes {          // which columns a lane holds
@@ -94,24 +134,30 @@ __global__ __launch_bounds__(kBlock) void norm_fwd_kernel(const T* __restrict__ 
     const int f = (L.lane + c * L.lpr) * V;
     f0[c] = f + V <= width ? f : width - V;
     skip[c] = f < width ? f - f0[c] : V;     // leading elements another lane owns
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      wv[c][k] = w && skip[c] < V ? w[f0[c] + k] : 1.f;
-      bv[c][k] = b && skip[c] < V ? b[f0[c] + k] : 0.f;
-    }
+    load_param<V>(w, f0[c], skip[c] < V, 1.f, wv[c]);
+    load_param<V>(b, f0[c], skip[c] < V, 0.f, bv[c]);
   }
   const float n = (float)width;   // a division: a constant row's mean stays exact
-  for (int64_t r0 = (int64_t)blockIdx.x * L.rows; r0 < rows; r0 += (int64_t)gridDim.x * L.rows) {
+  Raw<T, V> next[NCH];
+  auto fetch = [&](int64_t row) {
+    const T* xr = x + (row < rows ? row : rows - 1) * ldx;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c)
+      if (skip[c] < V) next[c].load(xr + f0[c]);
+  };
+  const int64_t stride = (int64_t)gridDim.x * L.rows;
+  fetch((int64_t)blockIdx.x * L.rows + L.row);
+  for (int64_t r0 = (int64_t)blockIdx.x * L.rows; r0 < rows; r0 += stride) {
     const int64_t row = r0 + L.row;
     const bool live = row < rows;
-    const T* xr = x + (live ? row : 0) * ldx;
     float v[NCH][V], sum = 0.f;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-      if (skip[c] < V) load_row<T, V>(xr + f0[c], v[c]);
+      next[c].get(v[c]);
 #pragma unroll
       for (int k = 0; k < V; ++k) sum += k >= skip[c] ? v[c][k] : 0.f;
     }
+    if (r0 + stride < rows) fetch(row + stride);   // over this row's sums
     const float mean = row_sum<WIDE>(sum, L.lpr, red, 0) / n;
     float sq = 0.f;
 #pragma unroll
@@ -155,51 +201,71 @@ __global__ __launch_bounds__(kBlock) void norm_bwd_kernel(const T* __restrict__ 
     const int f = (L.lane + c * L.lpr) * V;
     f0[c] = f + V <= width ? f : width - V;
     skip[c] = f < width ? f - f0[c] : V;
+    load_param<V>(w, f0[c], skip[c] < V, 1.f, wv[c]);
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      wv[c][k] = w && skip[c] < V ? w[f0[c] + k] : 1.f;
-      dw[c][k] = db[c][k] = 0.f;
-    }
+    for (int k = 0; k < V; ++k) dw[c][k] = db[c][k] = 0.f;
   }
   const float n = (float)width;
+  Raw<T, V> xn[NCH], gn[NCH];
+  float mean_n = 0.f, rstd_n = 0.f;
+  auto fetch = [&](int64_t row) {
+    const int64_t at = row < rows ? row : rows - 1;
+    mean_n = mean_in[at];
+    rstd_n = rstd_in[at];
+#pragma unroll
+    for (int c = 0; c < NCH; ++c)
+      if (skip[c] < V) {
+        xn[c].load(x + at * ldx + f0[c]);
+        gn[c].load(dy + at * lddy + f0[c]);
+      }
+  };
+  const int64_t stride = (int64_t)gridDim.x * L.rows;
+  if (rows > 0) fetch((int64_t)blockIdx.x * L.rows + L.row);
   int turn = 0;
-  for (int64_t r0 = (int64_t)blockIdx.x * L.rows; r0 < rows; r0 += (int64_t)gridDim.x * L.rows) {
+  for (int64_t r0 = (int64_t)blockIdx.x * L.rows; r0 < rows; r0 += stride) {
     const int64_t row = r0 + L.row;
     const bool live = row < rows;
-    const int64_t at = live ? row : 0;
-    const float mean = mean_in[at], rstd = rstd_in[at];
-    float xh[NCH][V], g[NCH][V], sg = 0.f, sgx = 0.f;
+    Raw<T, V> xr[NCH], gr[NCH];
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) xr[c] = xn[c], gr[c] = gn[c];
+    const float mean = mean_n, rstd = rstd_n;
+    if (r0 + stride < rows) fetch(row + stride);   // over this row's work
+    float sg = 0.f, sgx = 0.f;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-      if (skip[c] < V) {
-        load_row<T, V>(x + at * ldx + f0[c], xh[c]);
-        load_row<T, V>(dy + at * lddy + f0[c], g[c]);
-      }
+      float xh[V], g[V];
+      xr[c].get(xh);
+      gr[c].get(g);
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        xh[c][k] = (xh[c][k] - mean) * rstd;
+        xh[k] = (xh[k] - mean) * rstd;
         if (live && k >= skip[c]) {
-          dw[c][k] += g[c][k] * xh[c][k];
-          db[c][k] += g[c][k];
+          dw[c][k] += g[k] * xh[k];
+          db[c][k] += g[k];
         }
-        g[c][k] *= wv[c][k];
+        g[k] *= wv[c][k];
         if (k >= skip[c]) {
-          sg += g[c][k];
-          sgx += g[c][k] * xh[c][k];
+          sg += g[k];
+          sgx += g[k] * xh[k];
         }
       }
     }
     if (!dx) continue;
-    const float mg = row_sum<WIDE>(sg, L.lpr, red, turn) / n;
-    const float mgx = row_sum<WIDE>(sgx, L.lpr, red, turn + 1) / n;
-    turn ^= 2;
+    row_sum2<WIDE>(sg, sgx, L.lpr, red, turn);
+    const float mg = sg / n, mgx = sgx / n;
+    turn ^= 1;
     if (!live) continue;
+    // xhat and g again from the row's 16 bytes a chunk: holding them in fp32 costs
+    // 16 registers a chunk, and waves
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
       if (skip[c] >= V) continue;
-      float o[V];
+      float xh[V], g[V], o[V];
+      xr[c].get(xh);
+      gr[c].get(g);
 #pragma unroll
-      for (int k = 0; k < V; ++k) o[k] = rstd * (g[c][k] - mg - xh[c][k] * mgx);
+      for (int k = 0; k < V; ++k)
+        o[k] = rstd * (g[k] * wv[c][k] - mg - (xh[k] - mean) * rstd * mgx);
       store_row<T, V>(dx + row * (int64_t)width + f0[c], o);
     }
   }
@@ -331,17 +397,19 @@ __global__ __launch_bounds__(kSumCols* kSumRows) void norm_sum_kernel(const floa
   }
 }
 
-// Lanes and chunks of a row.  Up to 64 lanes x 4 chunks of 16 bytes a wave
-// owns it, then a workgroup up to 8192 elements; past that it is re-read.
+// Lanes and chunks of a row.  Up to 64 lanes x 4 chunks of 16 bytes a wave owns
+// it, then a workgroup up to 8192 elements; past that it is re-read.  The bf16
+// backward goes over to the workgroup at two chunks already: four hold 256
+// registers a lane (20011 x 2040: 64 us by waves, 54 us by workgroups).
 struct Shape {
   int v, lpr_log2, nch;
   bool wide, loop;
 };
-Shape shape_of(int dtype, int64_t width) {
+Shape shape_of(int dtype, int64_t width, bool backward) {
   const int full = dtype == SLDM_F32 ? 4 : 8;
   Shape s{width >= full ? full : 1, 0, 1, false, width > 8192};
   const int64_t need = (width + s.v - 1) / s.v;
-  if (need > 64 * 4) {
+  if (need > (backward && full == 8 ? 128 : 64 * 4)) {
     s.wide = true;
     s.lpr_log2 = 8;
   } else {
@@ -355,23 +423,27 @@ int64_t row_groups(const Shape& s, int64_t rows) {
   const int64_t per = kBlock >> s.lpr_log2;
   return (rows + per - 1) / per;
 }
-// Workgroups of the backward, each with a row of partial sums: four a CU, and
-// not so many that a workgroup's row of partials outweighs its rows.
+// Workgroups of the backward, each with a row of partial sums: enough to fill the
+// chip, few enough that wide rows of partials do not outweigh the rows (bf16,
+// 512 / 1024 / 2048 of them: 5003 x 8000 76 / 107 / 121 us, 100000 x 513 82 / 93 /
+// 83 us).
 int parts_of(const Shape& s, int64_t rows, int64_t width) {
   if (s.loop) return (int)std::max<int64_t>(1, std::min<int64_t>(rows, 64));
   const int64_t n = row_groups(s, rows);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(1024, std::max<int64_t>(n / 4, std::min<int64_t>(n, 256))));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(width > 512 ? 512 : 1024, std::max<int64_t>(n / 4, std::min<int64_t>(n, 256))));
 }
 
 template <typename T>
 void fwd(const T* x, int64_t ldx, int64_t rows, int64_t width, const float* w, const float* b, float eps, T* y,
          float* mean, float* rstd, hipStream_t st) {
-  const Shape s = shape_of(sizeof(T) == 4 ? SLDM_F32 : SLDM_BF16, width);
+  const Shape s = shape_of(sizeof(T) == 4 ? SLDM_F32 : SLDM_BF16, width, false);
   if (s.loop) {
     norm_fwd_long_kernel<T><<<(unsigned)rows, kBlock, 0, st>>>(x, ldx, width, w, b, eps, y, mean, rstd);
     return;
   }
-  const unsigned grid = (unsigned)std::min<int64_t>(row_groups(s, rows), 2048);
+  // rows enough a wave that reading w and b once pays (20011 x 2048 bf16, reading
+  // them for every two rows: 66 us; for five: 30 us)
+  const unsigned grid = (unsigned)std::min<int64_t>(row_groups(s, rows), s.nch == 1 ? 2048 : 1024);
   constexpr int F = 16 / sizeof(T);
 #define SLDM_GO(V, N, W) \
   norm_fwd_kernel<T, V, N, W><<<grid, kBlock, 0, st>>>(x, ldx, rows, (int)width, s.lpr_log2, w, b, eps, y, mean, rstd)
@@ -391,7 +463,7 @@ void fwd(const T* x, int64_t ldx, int64_t rows, int64_t width, const float* w, c
 template <typename T>
 void bwd(const T* x, int64_t ldx, const T* dy, int64_t lddy, int64_t rows, int64_t width, const float* w,
          const float* mean, const float* rstd, T* dx, float* dw, float* db, float* part, hipStream_t st) {
-  const Shape s = shape_of(sizeof(T) == 4 ? SLDM_F32 : SLDM_BF16, width);
+  const Shape s = shape_of(sizeof(T) == 4 ? SLDM_F32 : SLDM_BF16, width, true);
   const int parts = parts_of(s, rows, width);
   if (!dw && !db) part = nullptr;
   if (s.loop) {
@@ -406,7 +478,8 @@ void bwd(const T* x, int64_t ldx, const T* dy, int64_t lddy, int64_t rows, int64
                                                         rstd, dx, part)
     if (s.v == 1) SLDM_GO(1, 1, false);
     else if (s.wide) {
-      if (s.nch <= 2) SLDM_GO(F, 2, true);
+      if (s.nch == 1) SLDM_GO(F, 1, true);
+      else if (s.nch == 2) SLDM_GO(F, 2, true);
       else if (s.nch <= 4) SLDM_GO(F, 4, true);
       else if constexpr (F == 4) SLDM_GO(F, 8, true);
     } else {
@@ -449,7 +522,7 @@ extern "C" int sldm_layer_norm_fwd(int dtype, const void* x, int64_t ldx, int64_
 
 extern "C" size_t sldm_layer_norm_bwd_workspace_bytes(int dtype, int64_t rows, int64_t width) {
   if (check_args(dtype, rows, width) != SLDM_OK) return 0;
-  return (size_t)parts_of(shape_of(dtype, width), rows, width) * 2 * width * 4;
+  return (size_t)parts_of(shape_of(dtype, width, true), rows, width) * 2 * width * 4;
 }
 
 extern "C" int sldm_layer_norm_bwd(int dtype, const void* x, int64_t ldx, const void* dy, int64_t lddy,
