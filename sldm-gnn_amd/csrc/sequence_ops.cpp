@@ -82,19 +82,16 @@ Rows as_rows(const Tensor& x) {
   return {y, n, n > 1 ? y.stride(0) : w};
 }
 
-Tensor norm_fwd(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps, Tensor* mean,
-                Tensor* rstd) {
+// stats: [2, rows], the rows' means and 1 / sqrt(var + eps)
+Tensor norm_fwd(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps, Tensor* stats) {
   DeviceGuard guard(x.device());
   const Rows r = as_rows(x);
   Tensor y = at::empty(x.sizes(), x.options());
-  if (mean) {
-    *mean = at::empty({r.rows}, x.options().dtype(at::kFloat));
-    *rstd = at::empty({r.rows}, x.options().dtype(at::kFloat));
-  }
+  if (stats) *stats = at::empty({2, r.rows}, x.options().dtype(at::kFloat));
+  float* mean = stats ? fptr(*stats) : nullptr;
   const Tensor w = f32c(weight), b = f32c(bias);
   check(sldm_layer_norm_fwd(dtype_code(x, "layer_norm"), r.t.data_ptr(), r.ld, r.rows, x.size(-1), fptr(w), fptr(b),
-                            (float)eps, y.data_ptr(), mean ? fptr(*mean) : nullptr, rstd ? fptr(*rstd) : nullptr,
-                            stream_of(x)),
+                            (float)eps, y.data_ptr(), mean, mean ? mean + r.rows : nullptr, stream_of(x)),
         "sldm_layer_norm_fwd");
   return y;
 }
@@ -102,10 +99,10 @@ Tensor norm_fwd(const Tensor& x, const Tensor& weight, const Tensor& bias, doubl
 struct NormFn : torch::autograd::Function<NormFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const optional<Tensor>& weight,
                         const optional<Tensor>& bias, double eps) {
-    Tensor mean, rstd;
+    Tensor stats;
     const Tensor w = or_none(weight), b = or_none(bias);
-    Tensor y = norm_fwd(x, w, b, eps, &mean, &rstd);
-    ctx->save_for_backward({x, w, mean, rstd});
+    Tensor y = norm_fwd(x, w, b, eps, &stats);
+    ctx->save_for_backward({x, w, stats});
     ctx->saved_data["bias"] = b.defined() ? (int64_t)b.scalar_type() : (int64_t)-1;
     return y;
   }
@@ -122,19 +119,19 @@ struct NormFn : torch::autograd::Function<NormFn> {
     const Rows r = as_rows(x), g = as_rows(grads[0].scalar_type() == x.scalar_type() ? grads[0]
                                                                                        : grads[0].to(x.scalar_type()));
     const int code = dtype_code(x, "layer_norm");
-    Tensor dx, both, ws, dw, db;
+    Tensor dx, ws, dw, db;
     if (need_x) dx = at::empty(x.sizes(), x.options());
     const auto f32 = x.options().dtype(at::kFloat);
     const size_t bytes = sldm_layer_norm_bwd_workspace_bytes(code, r.rows, width);
     if (need_w || need_b) {
-      both = at::empty({2, width}, f32);
       ws = at::empty({(int64_t)(bytes / 4)}, f32);
-      if (need_w) dw = both[0];
-      if (need_b) db = both[1];
+      if (need_w) dw = at::empty({width}, f32);
+      if (need_b) db = at::empty({width}, f32);
     }
     const Tensor wf = f32c(w);
+    const float* mean = fptr(saved[2]);
     check(sldm_layer_norm_bwd(code, r.t.data_ptr(), r.ld, g.t.data_ptr(), g.ld, r.rows, width, fptr(wf),
-                              fptr(saved[2]), fptr(saved[3]), ptr(dx), fptr(dw), fptr(db), ptr(ws),
+                              mean, mean + r.rows, ptr(dx), fptr(dw), fptr(db), ptr(ws),
                               ws.defined() ? bytes : 0, stream_of(x)),
           "sldm_layer_norm_bwd");
     out[0] = dx;
@@ -159,7 +156,7 @@ Tensor layer_norm(const Tensor& x, const optional<Tensor>& weight, const optiona
   TORCH_CHECK_VALUE(eps >= 0, "layer_norm: eps must not be negative");
   require_gpu("layer_norm", x, {&w, &b});
   if (at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b))) return NormFn::apply(x, weight, bias, eps);
-  return norm_fwd(x, w, b, eps, nullptr, nullptr);
+  return norm_fwd(x, w, b, eps, nullptr);
 }
 
 // ------------------------------------------------------------------- rotary --
