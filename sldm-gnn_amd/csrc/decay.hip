@@ -14,11 +14,13 @@ constexpr int64_t kMaxThreads = (int64_t)1 << 32;   // work-items of one launch,
 constexpr int kChunk = 32;   // tokens of a segment are a multiple of this: no padding inside a sequence
 
 // Segments of the time axis.  One workgroup walks a sequence alone unless that
-// leaves the chip short of waves; then the axis is cut into pieces of at least 4
-// chunks, at the price of a pass over k and v for the pieces' states, which are
-// read and written too.  Waves aimed at, of 2048 / 3072 / 4096: bf16 (8 heads of
-// 128, 32768 frames, training) 365 / 397 / 438 us, fp32 (8 heads of 48 and 80,
-// 1237 frames, training) 264 / 221 / 211 us.
+// leaves the chip short of waves; then the axis is cut, at the price of a pass
+// over k and v for the pieces' states, which are read and written too.  Fewer
+// than four pieces do not pay for that pass (bf16, 64 heads of 64, 1024 frames:
+// 59 us whole, 54 us in two, 40 in four; 128 heads, 512 frames: 34, 40, 37), nor
+// do short ones.  Waves aimed at, of 2048 / 3072 / 4096: bf16 (8 heads of 128,
+// 32768 frames, training) 365 / 397 / 438 us, fp32 (8 heads of 48 and 80, 1237
+// frames, training) 264 / 221 / 211 us.
 struct Plan {
   int64_t seg_len;
   int nseg;
@@ -27,9 +29,10 @@ Plan plan(int dtype, int64_t B, int64_t H, int64_t T, int64_t dk, int64_t dv, in
   const int64_t C = kChunk;
   const int64_t waves = B * H * roles * std::max(tiles_of((int)dk), tiles_of((int)dv));
   const int64_t chunks = (T + C - 1) / C;
-  int64_t want = waves > 0 ? (dtype == SLDM_F32 ? 4096 : 2048) / waves : 1;
-  want = std::min(want, chunks / 4);
-  if (want <= 1) return {std::max<int64_t>(T, 1), 1};
+  const bool f32 = dtype == SLDM_F32;
+  int64_t want = waves > 0 ? (f32 ? 4096 : 2048) / waves : 1;
+  want = std::min(want, chunks / (f32 ? 4 : 8));
+  if (want < 4) return {std::max<int64_t>(T, 1), 1};
   const int64_t per = (chunks + want - 1) / want;
   return {per * C, (int)((chunks + per - 1) / per)};
 }

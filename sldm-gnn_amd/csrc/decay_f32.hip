@@ -246,7 +246,7 @@ void launch(const Args& a, hipStream_t st) {
 // of workgroups.
 template <int KT, bool OUT>
 void by_cols(const Args& a, int vd, hipStream_t st) {
-  constexpr int SUB = KT <= 2 ? 2 : 1;
+  constexpr int SUB = KT == 1 ? 2 : 1;
   if (vd <= 16) launch<KT, 1, 1, SUB, OUT>(a, st);
   else if (vd <= 32) launch<KT, 2, 1, SUB, OUT>(a, st);
   else if (vd <= 64) launch<KT, 2, 2, 1, OUT>(a, st);
