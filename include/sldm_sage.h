@@ -448,25 +448,31 @@ int sldm_rotary_axes(int dtype, const void* q, const int64_t* ld_q, int64_t head
  * lengths[b] on (clamped to [0, T]) are padding: not read into the state, their
  * outputs are zeros.  out [B, T, H, dv] contiguous.  1 <= dk, dv <= 128.
  * log_decay [H] fp32, <= 0 (-inf: nothing is kept).
- * workspace: sldm_decay_attention_workspace_bytes(.., backward). */
-size_t sldm_decay_attention_workspace_bytes(int dtype, int64_t B, int64_t T, int64_t H, int64_t Hk,
-                                            int64_t dk, int64_t dv, int backward);
+ * A long axis with few (batch, head) pairs is cut into segments; `states`
+ * (sldm_decay_attention_states_bytes bytes; 0: may be NULL) then takes the
+ * states before each, which the backward starts from. */
+size_t sldm_decay_attention_states_bytes(int dtype, int64_t B, int64_t T, int64_t H, int64_t Hk,
+                                         int64_t dk, int64_t dv);
 int sldm_decay_attention_fwd(int dtype, const void* q, const int64_t* ld_q, const void* k,
                              const int64_t* ld_k, const void* v, const int64_t* ld_v, int64_t B,
                              int64_t T, int64_t H, int64_t Hk, int64_t dk, int64_t dv,
                              const float* log_decay, float scale, const float* state,
                              const void* lengths, int lengths_int64, void* out, float* state_out,
-                             void* workspace, size_t workspace_bytes, void* stream);
+                             float* states, size_t states_bytes, void* stream);
 /* Gradients of sldm_decay_attention_fwd with respect to q, k, v and state
  * (contiguous, each nullable; padding tokens get zeros).  dout has `out`'s
  * shape with strides ld_do; dstate_out (nullable: zeros) is state_out's
- * gradient.  Shared key heads: the group's parts are added in fp32, in order. */
+ * gradient; `states` what the forward call of the same arguments wrote there.
+ * Shared key heads: the group's parts are added in fp32, in order. */
+size_t sldm_decay_attention_bwd_workspace_bytes(int dtype, int64_t B, int64_t T, int64_t H,
+                                                int64_t Hk, int64_t dk, int64_t dv);
 int sldm_decay_attention_bwd(int dtype, const void* q, const int64_t* ld_q, const void* k,
                              const int64_t* ld_k, const void* v, const int64_t* ld_v,
                              const void* dout, const int64_t* ld_do, int64_t B, int64_t T,
                              int64_t H, int64_t Hk, int64_t dk, int64_t dv,
                              const float* log_decay, float scale, const float* state,
-                             const float* dstate_out, const void* lengths, int lengths_int64,
+                             const float* states, const float* dstate_out, const void* lengths,
+                             int lengths_int64,
                              void* dq, void* dk_out, void* dv_out, float* dstate, void* workspace,
                              size_t workspace_bytes, void* stream);
 /* One token for each sequence, the state [B, H, dk, dv] moved on in place:

@@ -37,6 +37,22 @@ Plan plan(int dtype, int64_t B, int64_t H, int64_t T, int64_t dk, int64_t dv, in
   return {per * C, (int)((chunks + per - 1) / per)};
 }
 
+// The backward's three walks need fewer, longer segments: whole multiples of the
+// forward's, whose states they start from (m: forward segments in one of theirs).
+struct Plans {
+  Plan fwd, bwd;
+  int m;
+};
+Plans plans(int dtype, int64_t B, int64_t H, int64_t T, int64_t dk, int64_t dv) {
+  Plans p{plan(dtype, B, H, T, dk, dv, 1), plan(dtype, B, H, T, dk, dv, 3), 1};
+  if (p.fwd.nseg == 1) p.bwd = p.fwd;
+  if (p.bwd.nseg > 1) {
+    p.m = (int)std::max<int64_t>(1, (p.bwd.seg_len + p.fwd.seg_len / 2) / p.fwd.seg_len);
+    p.bwd = {p.fwd.seg_len * p.m, (p.fwd.nseg + p.m - 1) / p.m};
+  }
+  return p;
+}
+
 // loc[bh][s]: the states that segments add, each from zero -> the states
 // before each segment, and the state behind the last one.
 __global__ __launch_bounds__(256) void scan_kernel(float* loc, const float* s0, float* s1, Args a,
@@ -220,13 +236,20 @@ int check_shape(int dtype, int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t 
 
 using namespace sldm_decay;
 
-extern "C" size_t sldm_decay_attention_workspace_bytes(int dtype, int64_t B, int64_t T, int64_t H, int64_t Hk,
-                                                       int64_t dk, int64_t dv, int backward) {
+extern "C" size_t sldm_decay_attention_states_bytes(int dtype, int64_t B, int64_t T, int64_t H, int64_t Hk,
+                                                    int64_t dk, int64_t dv) {
   if (check_shape(dtype, B, T, H, Hk, dk, dv) != SLDM_OK) return 0;
-  const Plan p = plan(dtype, B, H, T, dk, dv, backward ? 3 : 1);
-  size_t n = p.nseg > 1 ? (size_t)(B * H) * p.nseg * dk * dv * (backward ? 2 : 1) : 0;
-  if (backward && H != Hk) n += (size_t)(B * T * H) * (dk + dv);
-  return n * 4 + 256;
+  const Plan p = plan(dtype, B, H, T, dk, dv, 1);
+  return p.nseg > 1 ? (size_t)(B * H) * p.nseg * dk * dv * 4 : 0;
+}
+
+extern "C" size_t sldm_decay_attention_bwd_workspace_bytes(int dtype, int64_t B, int64_t T, int64_t H, int64_t Hk,
+                                                           int64_t dk, int64_t dv) {
+  if (check_shape(dtype, B, T, H, Hk, dk, dv) != SLDM_OK) return 0;
+  const Plans p = plans(dtype, B, H, T, dk, dv);
+  size_t n = p.bwd.nseg > 1 ? (size_t)(B * H) * p.fwd.nseg * dk * dv : 0;
+  if (H != Hk) n += (size_t)(B * T * H) * (dk + dv);
+  return n * 4;
 }
 
 extern "C" int sldm_decay_attention_fwd(int dtype, const void* q, const int64_t* ld_q, const void* k,
@@ -234,13 +257,13 @@ extern "C" int sldm_decay_attention_fwd(int dtype, const void* q, const int64_t*
                                         int64_t T, int64_t H, int64_t Hk, int64_t dk, int64_t dv,
                                         const float* log_decay, float scale, const float* state,
                                         const void* lengths, int lengths_int64, void* out, float* state_out,
-                                        void* workspace, size_t workspace_bytes, void* stream) {
+                                        float* states, size_t states_bytes, void* stream) {
   if (const int rc = check_shape(dtype, B, T, H, Hk, dk, dv)) return rc;
   if (B == 0) return SLDM_OK;
   SLDM_REQUIRE(ld_q && ld_k && ld_v && log_decay, "sldm_decay_attention_fwd: null argument");
   SLDM_REQUIRE(T == 0 || (q && k && v && out), "sldm_decay_attention_fwd: null argument");
-  SLDM_REQUIRE(workspace_bytes >= sldm_decay_attention_workspace_bytes(dtype, B, T, H, Hk, dk, dv, 0) && workspace,
-               "sldm_decay_attention_fwd: workspace too small");
+  const size_t need = sldm_decay_attention_states_bytes(dtype, B, T, H, Hk, dk, dv);
+  SLDM_REQUIRE(!need || (states && states_bytes >= need), "sldm_decay_attention_fwd: no room for the states");
   const int esz = dtype == SLDM_F32 ? 4 : 2, group = (int)(H / Hk);
   const Plan p = plan(dtype, B, H, T, dk, dv, 1);
   const int64_t elems = dk * dv;
@@ -266,7 +289,7 @@ extern "C" int sldm_decay_attention_fwd(int dtype, const void* q, const int64_t*
     SLDM_LAUNCH_CHECK("decay_kernel");
     return SLDM_OK;
   }
-  float* loc = reinterpret_cast<float*>(workspace);
+  float* loc = states;
   r.s1 = loc; r.s1_bh = p.nseg * elems; r.s1_seg = elems;
   launch_roles(dtype, a, one, 1, false, st);
   SLDM_LAUNCH_CHECK("decay_kernel (states)");
@@ -282,29 +305,32 @@ extern "C" int sldm_decay_attention_bwd(int dtype, const void* q, const int64_t*
                                         const int64_t* ld_k, const void* v, const int64_t* ld_v, const void* dout,
                                         const int64_t* ld_do, int64_t B, int64_t T, int64_t H, int64_t Hk,
                                         int64_t dk, int64_t dv, const float* log_decay, float scale,
-                                        const float* state, const float* dstate_out, const void* lengths,
-                                        int lengths_int64, void* dq, void* dk_out, void* dv_out, float* dstate,
-                                        void* workspace, size_t workspace_bytes, void* stream) {
+                                        const float* state, const float* states, const float* dstate_out,
+                                        const void* lengths, int lengths_int64, void* dq, void* dk_out, void* dv_out,
+                                        float* dstate, void* workspace, size_t workspace_bytes, void* stream) {
   if (const int rc = check_shape(dtype, B, T, H, Hk, dk, dv)) return rc;
   if (B == 0) return SLDM_OK;
   SLDM_REQUIRE(ld_q && ld_k && ld_v && ld_do && log_decay, "sldm_decay_attention_bwd: null argument");
   SLDM_REQUIRE(T == 0 || (q && k && v && dout), "sldm_decay_attention_bwd: null argument");
-  SLDM_REQUIRE(workspace_bytes >= sldm_decay_attention_workspace_bytes(dtype, B, T, H, Hk, dk, dv, 1) && workspace,
-               "sldm_decay_attention_bwd: workspace too small");
+  const size_t need = sldm_decay_attention_bwd_workspace_bytes(dtype, B, T, H, Hk, dk, dv);
+  SLDM_REQUIRE(!need || (workspace && workspace_bytes >= need), "sldm_decay_attention_bwd: workspace too small");
   const int esz = dtype == SLDM_F32 ? 4 : 2, group = (int)(H / Hk);
-  const Plan p = plan(dtype, B, H, T, dk, dv, 3);
+  const Plans p = plans(dtype, B, H, T, dk, dv);
+  const bool cut = p.bwd.nseg > 1;
+  SLDM_REQUIRE(!cut || states, "sldm_decay_attention_bwd: the forward's states are needed");
   const int64_t elems = dk * dv;
   hipStream_t st = sldm::as_stream(stream);
   Args a{};
   a.B = B; a.H = H; a.T = T;
-  a.seg_len = p.seg_len; a.nseg = p.nseg; a.groups = (int)(B * H * p.nseg);
   a.log_decay = log_decay; a.lengths = lengths; a.lengths64 = lengths_int64;
+  auto segments = [&](const Plan& s) {
+    a.seg_len = s.seg_len; a.nseg = s.nseg; a.groups = (int)(B * H * s.nseg);
+  };
 
   float* ws = reinterpret_cast<float*>(workspace);
-  float *locS = nullptr, *locR = nullptr, *part_k = nullptr, *part_v = nullptr;
-  if (p.nseg > 1) {
-    locS = ws; ws += B * H * p.nseg * elems;
-    locR = ws; ws += B * H * p.nseg * elems;
+  float *locR = nullptr, *part_k = nullptr, *part_v = nullptr;
+  if (cut) {
+    locR = ws; ws += B * H * p.fwd.nseg * elems;
   }
   if (group > 1) {
     part_k = ws; ws += B * T * H * dk;
@@ -332,29 +358,24 @@ extern "C" int sldm_decay_attention_bwd(int dtype, const void* q, const int64_t*
   rk.delta = rk.reverse = 1;
   set_out(rk, group > 1 ? (void*)part_k : dk_out, T, H, dk, group > 1, esz);
 
-  if (p.nseg > 1) {
-    Role s{}, g = rv;                            // states that each segment adds
-    s.k = ok; s.v = ov;
-    s.kd = (int)dk; s.vd = (int)dv;
-    s.s_k = dv; s.s_v = 1;
-    s.upd_scale = 1.f;
-    s.s1 = locS; g.s1 = locR;
-    s.s1_bh = g.s1_bh = p.nseg * elems;
-    s.s1_seg = g.s1_seg = elems;
-    const Role* two[2];
-    int n = 0;
-    if (dq) two[n++] = &s;
-    if (dk_out || dv_out || dstate) two[n++] = &g;
-    launch_roles(dtype, a, two, n, false, st);
-    SLDM_LAUNCH_CHECK("decay_kernel (states)");
-    if (dq)
-      if (const int rc = scan(locS, state, nullptr, a, elems, st)) return rc;
-    if (dk_out || dv_out || dstate)
+  if (cut) {
+    if (dk_out || dv_out || dstate) {            // the gradient that each segment adds to the state
+      segments(p.fwd);
+      Role g = rv;
+      g.s1 = locR;
+      g.s1_bh = p.fwd.nseg * elems;
+      g.s1_seg = elems;
+      const Role* one[1] = {&g};
+      launch_roles(dtype, a, one, 1, false, st);
+      SLDM_LAUNCH_CHECK("decay_kernel (states)");
       if (const int rc = scan(locR, dstate_out, dstate, a, elems, st)) return rc;
-    rq.s0 = locS; rk.s0 = rv.s0 = locR;
-    rq.s0_bh = rk.s0_bh = rv.s0_bh = p.nseg * elems;
-    rq.s0_seg = rk.s0_seg = rv.s0_seg = elems;
+    }
+    segments(p.bwd);
+    rq.s0 = states; rk.s0 = rv.s0 = locR;
+    rq.s0_bh = rk.s0_bh = rv.s0_bh = p.fwd.nseg * elems;
+    rq.s0_seg = rk.s0_seg = rv.s0_seg = p.m * elems;
   } else {
+    segments(p.bwd);
     rq.s0 = state; rk.s0 = rv.s0 = dstate_out;
     rq.s0_bh = rk.s0_bh = rv.s0_bh = elems;
     rv.s1 = dstate; rv.s1_bh = elems;

@@ -316,34 +316,31 @@ struct Ld {
   int64_t s[3];
   explicit Ld(const Tensor& t) : s{t.stride(0), t.stride(1), t.stride(2)} {}
 };
-// offsets of rows nobody reads do not matter: an empty tensor's pointer may be null
-struct Work {
-  Tensor t;
-  size_t bytes;
-  Work(const Tensor& like, const Dims& d, bool backward) {
-    bytes = sldm_decay_attention_workspace_bytes(dtype_code(like, "decay_attention"), d.B, d.T, d.H, d.Hk, d.dk, d.dv,
-                                                 backward);
-    t = at::empty({(int64_t)(bytes / 4)}, like.options().dtype(at::kFloat));
-  }
-};
 Dims dims_of(const Tensor& q, const Tensor& k, const Tensor& v) {
   return {q.size(0), q.size(1), q.size(2), k.size(2), q.size(3), v.size(3)};
 }
 
-std::pair<Tensor, Tensor> attend(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay,
-                                 const Tensor& state, const Tensor& lengths, double scale) {
+struct Attended {
+  Tensor out, end, states;     // states: before each segment of a long axis (for the backward)
+};
+Attended attend(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Tensor& state,
+                const Tensor& lengths, double scale) {
   DeviceGuard guard(q.device());
   const Dims d = dims_of(q, k, v);
-  Tensor out = at::empty({d.B, d.T, d.H, d.dv}, q.options());
-  Tensor end = at::empty({d.B, d.H, d.dk, d.dv}, q.options().dtype(at::kFloat));
-  const Work w(q, d, false);
+  const int code = dtype_code(q, "decay_attention");
+  const auto f32 = q.options().dtype(at::kFloat);
+  Attended r;
+  r.out = at::empty({d.B, d.T, d.H, d.dv}, q.options());
+  r.end = at::empty({d.B, d.H, d.dk, d.dv}, f32);
+  const size_t bytes = sldm_decay_attention_states_bytes(code, d.B, d.T, d.H, d.Hk, d.dk, d.dv);
+  if (bytes) r.states = at::empty({(int64_t)(bytes / 4)}, f32);
   const Ld lq(q), lk(k), lv(v);
-  check(sldm_decay_attention_fwd(dtype_code(q, "decay_attention"), q.data_ptr(), lq.s, k.data_ptr(), lk.s, v.data_ptr(),
-                                 lv.s, d.B, d.T, d.H, d.Hk, d.dk, d.dv, fptr(log_decay), (float)scale, fptr(state),
-                                 ptr(lengths), lengths.defined() && lengths.scalar_type() == at::kLong, out.data_ptr(),
-                                 fptr(end), w.t.data_ptr(), w.bytes, stream_of(q)),
+  check(sldm_decay_attention_fwd(code, q.data_ptr(), lq.s, k.data_ptr(), lk.s, v.data_ptr(), lv.s, d.B, d.T, d.H, d.Hk,
+                                 d.dk, d.dv, fptr(log_decay), (float)scale, fptr(state), ptr(lengths),
+                                 lengths.defined() && lengths.scalar_type() == at::kLong, r.out.data_ptr(), fptr(r.end),
+                                 fptr(r.states), bytes, stream_of(q)),
         "sldm_decay_attention_fwd");
-  return {out, end};
+  return r;
 }
 
 struct DecayFn : torch::autograd::Function<DecayFn> {
@@ -354,9 +351,9 @@ struct DecayFn : torch::autograd::Function<DecayFn> {
     const Tensor q = cols(q_in), k = cols(k_in), v = cols(v_in), g = log_decay.contiguous(), lengths = or_none(lengths_in);
     const Tensor state = given(state_in) ? state_in->contiguous() : Tensor();
     const auto r = attend(q, k, v, g, state, lengths, scale);
-    ctx->save_for_backward({q, k, v, g, state, lengths});
+    ctx->save_for_backward({q, k, v, g, state, lengths, r.states});
     ctx->saved_data["scale"] = scale;
-    return {r.first, r.second};
+    return {r.out, r.end};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once("decay_attention");
@@ -374,13 +371,17 @@ struct DecayFn : torch::autograd::Function<DecayFn> {
     if (ctx->needs_input_grad(1)) dk = at::empty(k.sizes(), k.options());
     if (ctx->needs_input_grad(2)) dv = at::empty(v.sizes(), v.options());
     if (state.defined() && ctx->needs_input_grad(4)) ds = at::empty(state.sizes(), state.options());
-    const Work w(q, d, true);
+    const int code = dtype_code(q, "decay_attention");
+    const size_t bytes = sldm_decay_attention_bwd_workspace_bytes(code, d.B, d.T, d.H, d.Hk, d.dk, d.dv);
+    Tensor ws;
+    if (bytes) ws = at::empty({(int64_t)(bytes / 4)}, q.options().dtype(at::kFloat));
     const Ld lq(q), lk(k), lv(v), ld(dout);
-    check(sldm_decay_attention_bwd(dtype_code(q, "decay_attention"), q.data_ptr(), lq.s, k.data_ptr(), lk.s,
+    check(sldm_decay_attention_bwd(code, q.data_ptr(), lq.s, k.data_ptr(), lk.s,
                                    v.data_ptr(), lv.s, dout.data_ptr(), ld.s, d.B, d.T, d.H, d.Hk, d.dk, d.dv, fptr(g),
-                                   (float)ctx->saved_data["scale"].toDouble(), fptr(state), fptr(dend), ptr(lengths),
+                                   (float)ctx->saved_data["scale"].toDouble(), fptr(state), fptr(saved[6]),
+                                   fptr(dend), ptr(lengths),
                                    lengths.defined() && lengths.scalar_type() == at::kLong, ptr(dq), ptr(dk), ptr(dv),
-                                   fptr(ds), w.t.data_ptr(), w.bytes, stream_of(q)),
+                                   fptr(ds), ptr(ws), bytes, stream_of(q)),
           "sldm_decay_attention_bwd");
     out[0] = dq;
     out[1] = dk;
@@ -414,7 +415,7 @@ std::tuple<Tensor, Tensor> decay_attention(const Tensor& q, const Tensor& k, con
   }
   auto r = attend(cols(q), cols(k), cols(v), log_decay.contiguous(), state.defined() ? state.contiguous() : state,
                   or_none(lens), scale);
-  return {r.first, r.second};
+  return {r.out, r.end};
 }
 
 Tensor decay_attention_step(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& log_decay,

@@ -116,16 +116,18 @@ _SIGNATURES = {
     "sldm_rotary_axes": (ctypes.c_int, [ctypes.c_int, _vp, _vp, _c_i64, _vp, _vp, _c_i64, _c_i64,
                                         _c_i64, _c_i64, _vp, ctypes.c_int, _vp, _vp, _vp, _c_i64,
                                         ctypes.c_int, ctypes.c_int, _vp, _vp, _vp]),
-    "sldm_decay_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int, _c_i64, _c_i64,
-                                                               _c_i64, _c_i64, _c_i64, _c_i64,
-                                                               ctypes.c_int]),
+    "sldm_decay_attention_states_bytes": (ctypes.c_size_t, [ctypes.c_int, _c_i64, _c_i64, _c_i64,
+                                                            _c_i64, _c_i64, _c_i64]),
+    "sldm_decay_attention_bwd_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int, _c_i64, _c_i64,
+                                                                   _c_i64, _c_i64, _c_i64,
+                                                                   _c_i64]),
     "sldm_decay_attention_fwd": (ctypes.c_int, [ctypes.c_int, _vp, _vp, _vp, _vp, _vp, _vp, _c_i64,
                                                 _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp,
                                                 ctypes.c_float, _vp, _vp, ctypes.c_int, _vp, _vp,
                                                 _vp, ctypes.c_size_t, _vp]),
     "sldm_decay_attention_bwd": (ctypes.c_int, [ctypes.c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                                 _vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,
-                                                _c_i64, _vp, ctypes.c_float, _vp, _vp, _vp,
+                                                _c_i64, _vp, ctypes.c_float, _vp, _vp, _vp, _vp,
                                                 ctypes.c_int, _vp, _vp, _vp, _vp, _vp,
                                                 ctypes.c_size_t, _vp]),
     "sldm_decay_attention_step": (ctypes.c_int, [ctypes.c_int, _vp, _vp, _vp, _vp, _vp, _vp,

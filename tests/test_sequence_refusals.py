@@ -134,7 +134,7 @@ def test_c_entries_refuse_before_any_launch():
     assert lib.sldm_layer_norm_fwd(0, None, 8, 4, 0, None, None, 1e-5, None, None, None, None) == 1
     assert lib.sldm_layer_norm_bwd(0, None, 8, None, 8, 4, 8, None, None, None, None, None, None, None, 0, None) == 0
     assert lib.sldm_layer_norm_bwd_workspace_bytes(0, 4, 8) > 0
-    assert lib.sldm_decay_attention_workspace_bytes(0, 1, 10, 2, 2, 200, 16, 0) == 0
+    assert lib.sldm_decay_attention_states_bytes(0, 1, 10, 2, 2, 200, 16) == 0
     assert b"head sizes" in lib.sldm_last_error()
     assert lib.sldm_decay_attention_fwd(0, None, None, None, None, None, None, 1, 4, 2, 2, 16, 16, None, 1.0, None,
                                         None, 0, None, None, None, 0, None) == 1
@@ -142,4 +142,6 @@ def test_c_entries_refuse_before_any_launch():
                                          None, None) == 1
     assert b"3 heads over 2" in lib.sldm_last_error()
     # long axes need room for their segments' states
-    assert lib.sldm_decay_attention_workspace_bytes(1, 1, 100000, 1, 1, 64, 64, 0) > 64 * 64 * 4 * 8
+    assert lib.sldm_decay_attention_states_bytes(1, 1, 100000, 1, 1, 64, 64) > 64 * 64 * 4 * 8
+    assert lib.sldm_decay_attention_bwd_workspace_bytes(1, 1, 100000, 1, 1, 64, 64) > 64 * 64 * 4 * 8
+    assert lib.sldm_decay_attention_states_bytes(1, 4096, 100, 6, 6, 16, 16) == 0
