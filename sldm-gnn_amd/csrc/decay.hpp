@@ -83,22 +83,26 @@ __device__ __forceinline__ int xcd_order(int unit) {
   return (turn * 8 + (((int)blockIdx.x + turn) & 7)) * unit + slot % unit;
 }
 
-// What a (batch, head, segment) is made of.
+// What a (batch, head, segment) is made of.  All uniform, and said so: what comes
+// from a vector load would otherwise live in vector registers.
 struct Span {
-  int64_t bh, b, hd, len, seg0, n, base;   // n: the segment's tokens; base: position x is token base +- x
+  int64_t bh, b;
+  int hd, len, seg0, n, base;   // n: the segment's tokens; base: position x is token base +- x
+  float ld2;                    // log2 of the decay
 };
 __device__ __forceinline__ Span span_of(const Args& a, const Role& R, int id) {
   Span s;
   const int per = a.groups / a.nseg;
-  const int seg = id / per;
+  const int seg = id / per, H = (int)a.H;
   s.bh = id % per;
-  s.b = s.bh / a.H;
-  s.hd = s.bh % a.H;
-  s.len = seq_len(a, s.b);
-  s.seg0 = (int64_t)seg * a.seg_len;
-  const int64_t left = s.len - s.seg0;
-  s.n = left < 0 ? 0 : (left < a.seg_len ? left : a.seg_len);
+  s.b = (int)s.bh / H;
+  s.hd = (int)s.bh % H;
+  s.len = __builtin_amdgcn_readfirstlane((int)seq_len(a, s.b));
+  s.seg0 = seg * (int)a.seg_len;
+  const int left = s.len - s.seg0, whole = (int)a.seg_len;
+  s.n = left < 0 ? 0 : (left < whole ? left : whole);
   s.base = R.reverse ? s.len - 1 - s.seg0 : s.seg0;
+  s.ld2 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(a.log_decay[s.hd]))) * 1.44269504088896340736f;
   return s;
 }
 
@@ -121,10 +125,10 @@ struct Tile {
   static __device__ __forceinline__ int row_of(int i) {
     return (i * NW + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * STEP + (int)(threadIdx.x & 63) / GR;
   }
-  __device__ __forceinline__ void init(const Operand& t, const T* head, const Span& s, int64_t sign, int pad, int d) {
+  __device__ __forceinline__ void init(const Operand& t, const T* head, const Span& s, int sign, int pad, int d) {
     const int64_t st = t.st;
-    base = reinterpret_cast<const char*>(head + (s.base - sign * pad + (sign < 0 ? -(ROWS - 1) : 0)) * st);
-    step = sign * ROWS * st * (int)sizeof(T);
+    base = reinterpret_cast<const char*>(head + (int64_t)(s.base - sign * pad + (sign < 0 ? -(ROWS - 1) : 0)) * st);
+    step = (int64_t)sign * ROWS * st * (int)sizeof(T);
     on = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -134,7 +138,7 @@ struct Tile {
     }
   }
   // chunk c, rows from `first` on, to LDS address `lds`
-  __device__ __forceinline__ void load(int64_t c, uint32_t lds, int first) const {
+  __device__ __forceinline__ void load(int c, uint32_t lds, int first) const {
     const char* p = base + c * step;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
@@ -145,12 +149,12 @@ struct Tile {
                      : "memory", "m0");
   }
   // any alignment: element by element; row r is position x0 + r (below 0: zeros)
-  static __device__ __forceinline__ void slow(char* lds, const T* row0, int64_t st, int64_t x0, int d) {
+  static __device__ __forceinline__ void slow(char* lds, const T* row0, int64_t st, int x0, int d) {
     constexpr int W = RB / (int)sizeof(T);
 #pragma unroll 1
     for (int i = threadIdx.x; i < ROWS * W; i += 64 * NW) {
       const int r = i / W, e = i % W;
-      const int64_t x = x0 + r;
+      const int x = x0 + r;
       *reinterpret_cast<T*>(lds + r * RB + ((e / E ^ SWZ<RB>::of(r)) << 4) + (int)sizeof(T) * (e % E)) =
           x >= 0 && e < d ? row0[x * st + e] : T(0);
     }
@@ -161,14 +165,14 @@ struct Tile {
 // thread where the rows allow it.
 template <int NTH, bool FAST>
 __device__ __forceinline__ void zero_tail(const Args& a, const Role& R, const Span& s, int elem_bytes) {
-  const int64_t t1 = s.seg0 + a.seg_len < a.T ? s.seg0 + a.seg_len : a.T;
-  const int64_t t0 = s.len > s.seg0 ? s.len : s.seg0;
+  const int T = (int)a.T, whole = (int)a.seg_len, t1 = T - s.seg0 > whole ? s.seg0 + whole : T;
+  const int t0 = s.len > s.seg0 ? s.len : s.seg0;
   if (t0 >= t1) return;
   constexpr int kLanes = 32;                     // across a row (of at most 512 bytes: 32 granules)
   const int col = (int)threadIdx.x % kLanes, bytes = R.vd * elem_bytes;
   char* o = reinterpret_cast<char*>(R.o) + (s.b * R.o_sb + s.hd * R.o_sh) * elem_bytes;
-  for (int64_t t = t0 + (int)threadIdx.x / kLanes; t < t1; t += NTH / kLanes) {
-    char* row = o + t * R.o_st * elem_bytes;
+  for (int t = t0 + (int)threadIdx.x / kLanes; t < t1; t += NTH / kLanes) {
+    char* row = o + (int64_t)t * R.o_st * elem_bytes;
     if (FAST) {
       if (16 * col < bytes) *reinterpret_cast<uint4*>(row + 16 * col) = make_uint4(0, 0, 0, 0);
     } else {

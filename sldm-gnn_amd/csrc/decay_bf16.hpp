@@ -147,16 +147,14 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_bf16_kernel(Ar
 
   const int order = xcd_order(a.unit), id = order / a.roles;
   if (id >= a.groups) return;
-  const Role& R = a.role[order % a.roles];
+  const Role R = a.role[order % a.roles];
   const Span sp = span_of(a, R, id);
-  const int seg = (int)(sp.seg0 / a.seg_len);
+  const int seg = sp.seg0 / (int)a.seg_len;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 31, h = lane >> 5;
   const int kd = R.kd, vd = R.vd;
-  const int pad = (int)((C - sp.n % C) % C);
-  const int64_t nch = (sp.n + pad) / C;
-  const float ld2 = a.log_decay[sp.hd] * 1.44269504088896340736f;
-  const int64_t sign = R.reverse ? -1 : 1;
+  const int pad = (C - sp.n % C) % C, nch = (sp.n + pad) / C, sign = R.reverse ? -1 : 1;
+  const float ld2 = sp.ld2;
 
   const uint16_t* qh = OUT ? reinterpret_cast<const uint16_t*>(R.q.p) + sp.b * R.q.sb + (sp.hd / R.q.hdiv) * R.q.sh : nullptr;
   const uint16_t* kh = reinterpret_cast<const uint16_t*>(R.k.p) + sp.b * R.k.sb + (sp.hd / R.k.hdiv) * R.k.sh;
@@ -165,7 +163,7 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_bf16_kernel(Ar
   TK tq, tk;
   TV tv;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_vptr)tiles;
-  auto fetch = [&](int64_t c, int first) {
+  auto fetch = [&](int c, int first) {
     const uint32_t at = lds0 + (uint32_t)(c & 1) * kBuf;
     tk.load(c, at, first);
     tv.load(c, at + TK::BYTES, first);
@@ -212,18 +210,23 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_bf16_kernel(Ar
   const float* pw = wtab + 8 * h;
   f16v O;
   // chunk c's outputs: lane = token m, registers 8 s + e = columns 16 s + 8 h + e
-  auto put = [&](int64_t c) {
-    const int64_t x = c * C + m - pad;
-    if (x < 0) return;
-    const int64_t off = sp.b * R.o_sb + (sp.base + sign * x) * R.o_st + sp.hd * R.o_sh + 32 * wave + 8 * h;
+  const int o_bytes = R.o_f32 ? 4 : 2;
+  char* o_at = OUT ? reinterpret_cast<char*>(R.o) + (sp.b * R.o_sb + (int64_t)(sp.base + sign * (m - pad)) * R.o_st +
+                                                     sp.hd * R.o_sh + 32 * wave + 8 * h) * o_bytes
+                   : nullptr;
+  const int64_t o_step = (int64_t)sign * C * R.o_st * o_bytes;
+  auto put = [&](int c) {
+    char* at = o_at;
+    o_at += o_step;
+    if (c * C + m < pad) return;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int c0 = 32 * wave + 16 * s + 8 * h;
       float y[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] = O[8 * s + e];
-      if (R.o_f32) {
-        float* o = reinterpret_cast<float*>(R.o) + off + 16 * s;
+      if (o_bytes == 4) {
+        float* o = reinterpret_cast<float*>(at) + 16 * s;
         if (FAST) {
           if (c0 < vd) {
             sldm::Vec<float, 4>::store(o, y);
@@ -235,7 +238,7 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_bf16_kernel(Ar
             if (c0 + e < vd) o[e] = y[e];
         }
       } else {
-        uint16_t* o = reinterpret_cast<uint16_t*>(R.o) + off + 16 * s;
+        uint16_t* o = reinterpret_cast<uint16_t*>(at) + 16 * s;
         if (FAST) {
           if (c0 < vd) sldm::Vec<uint16_t, 8>::store(o, y);
         } else {
@@ -246,8 +249,11 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_bf16_kernel(Ar
       }
     }
   };
+  // the first chunk's padding shortens what lies between the state and its rows
+  const float rd_full = powg(ld2, m + 1 - R.delta) * R.read_scale, gn_full = powg(ld2, C);
+  float rd = powg(ld2, m - pad + 1 - R.delta) * R.read_scale, gn = powg(ld2, C - pad);
 
-  for (int64_t c = 0; c < nch; ++c) {
+  for (int c = 0; c < nch; ++c) {
     if constexpr (FAST) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // this chunk's tiles (and older stores)
       __syncthreads();                                          // of all waves; the other buffer is free
@@ -256,11 +262,11 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_bf16_kernel(Ar
     } else {
       if (OUT && c > 0) put(c - 1);
       __syncthreads();
-      const int64_t x0 = c * C - pad;
+      const int x0 = c * C - pad;
       char* at = tiles + (c & 1) * kBuf;
-      TK::slow(at, kh + sp.base * R.k.st, sign * R.k.st, x0, kd);
-      TV::slow(at + TK::BYTES, vh + sp.base * R.v.st, sign * R.v.st, x0, vd);
-      if constexpr (OUT) TK::slow(at + TK::BYTES + TV::BYTES, qh + sp.base * R.q.st, sign * R.q.st, x0, kd);
+      TK::slow(at, kh + (int64_t)sp.base * R.k.st, sign * R.k.st, x0, kd);
+      TV::slow(at + TK::BYTES, vh + (int64_t)sp.base * R.v.st, sign * R.v.st, x0, vd);
+      if constexpr (OUT) TK::slow(at + TK::BYTES + TV::BYTES, qh + (int64_t)sp.base * R.q.st, sign * R.q.st, x0, kd);
       __syncthreads();
     }
     // the tables are read, and the operands' places worked out, anew: not kept in registers
@@ -268,7 +274,6 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_bf16_kernel(Ar
     const char* lk = tiles + (c & 1) * kBuf;
     const char* lv = lk + TK::BYTES;
     const char* lq = lv + TV::BYTES;
-    const int padc = c == 0 ? pad : 0;
     bf8v vf[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) vf[s] = cv.at<RBV>(lv, wave, s);
@@ -297,7 +302,6 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_bf16_kernel(Ar
         P = mfma(kf, qf, P);
         phase();
       }
-      const float rd = powg(ld2, m - padc + 1 - R.delta) * R.read_scale;
 #pragma unroll
       for (int r = 0; r < 16; ++r) O[r] *= rd;
 #pragma unroll
@@ -315,8 +319,9 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_bf16_kernel(Ar
         }
       }
     }
-    const float gn = powg(ld2, C - padc);
     update<KT, EXACT ? 3 : 2>(S, vf, lk, ck, pw, gn);
+    rd = rd_full;
+    gn = gn_full;
   }
   if (OUT && nch > 0) put(nch - 1);
   if (R.s1) {

@@ -45,16 +45,14 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_f32_kernel(Arg
 
   const int order = xcd_order(a.unit), id = order / a.roles;
   if (id >= a.groups) return;
-  const Role& R = a.role[order % a.roles];
+  const Role R = a.role[order % a.roles];
   const Span sp = span_of(a, R, id);
-  const int seg = (int)(sp.seg0 / a.seg_len);
+  const int seg = sp.seg0 / (int)a.seg_len;
   const int lane = threadIdx.x & 63, m = lane & 15, h = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), v0 = 16 * NV * wave;
   const int kd = R.kd, vd = R.vd;
-  const int pad = (int)((ROWS - sp.n % ROWS) % ROWS);
-  const int64_t nt = (sp.n + pad) / ROWS;
-  const int64_t sign = R.reverse ? -1 : 1;
-  const float ld2 = a.log_decay[sp.hd] * 1.44269504088896340736f;
+  const int pad = (ROWS - sp.n % ROWS) % ROWS, nt = (sp.n + pad) / ROWS, sign = R.reverse ? -1 : 1;
+  const float ld2 = sp.ld2;
 
   const float* qh = OUT ? reinterpret_cast<const float*>(R.q.p) + sp.b * R.q.sb + (sp.hd / R.q.hdiv) * R.q.sh : nullptr;
   const float* kh = reinterpret_cast<const float*>(R.k.p) + sp.b * R.k.sb + (sp.hd / R.k.hdiv) * R.k.sh;
@@ -63,7 +61,7 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_f32_kernel(Arg
   TK tq, tk;
   TV tv;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_vptr)tiles;
-  auto fetch = [&](int64_t c, int first) {
+  auto fetch = [&](int c, int first) {
     const uint32_t at = lds0 + (uint32_t)(c & 1) * kBuf;
     tk.load(c, at, first);
     tv.load(c, at + TK::BYTES, first);
@@ -113,27 +111,31 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_f32_kernel(Arg
   int row_x = (h ^ Swizzle<RBK>::of(m)) << 4, kcol_x = (m >> 2 ^ Swizzle<RBK>::of(4 * h)) << 4;
   const int vcol_x = (m >> 2 ^ Swizzle<RBV>::of(4 * h)) << 4;
   f4v O[SUB][NV];
-  auto put = [&](int64_t c) {
+  float* o_at = OUT ? reinterpret_cast<float*>(R.o) + sp.b * R.o_sb + (int64_t)(sp.base + sign * (m - pad)) * R.o_st +
+                          sp.hd * R.o_sh + v0 + 4 * h
+                    : nullptr;
+  const int64_t o_step = (int64_t)sign * C * R.o_st;
+  auto put = [&](int c) {
 #pragma unroll
     for (int s = 0; s < SUB; ++s) {
-      const int64_t x = c * ROWS + C * s + m - pad;
-      if (x < 0) continue;
-      float* o = reinterpret_cast<float*>(R.o) + sp.b * R.o_sb + (sp.base + sign * x) * R.o_st + sp.hd * R.o_sh;
+      float* o = o_at;
+      o_at += o_step;
+      if (c * ROWS + C * s + m < pad) continue;
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         const int c0 = v0 + 16 * v + 4 * h;
         if (FAST) {
-          if (c0 < vd) *reinterpret_cast<f4v*>(o + c0) = O[s][v];
+          if (c0 < vd) *reinterpret_cast<f4v*>(o + 16 * v) = O[s][v];
         } else {
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (c0 + r < vd) o[c0 + r] = O[s][v][r];
+            if (c0 + r < vd) o[16 * v + r] = O[s][v][r];
         }
       }
     }
   };
 
-  for (int64_t c = 0; c < nt; ++c) {
+  for (int c = 0; c < nt; ++c) {
     if constexpr (FAST) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // this tile (and older stores)
       __syncthreads();                                          // of all waves; the other buffer is free
@@ -142,11 +144,11 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_f32_kernel(Arg
     } else {
       if (OUT && c > 0) put(c - 1);
       __syncthreads();
-      const int64_t x0 = c * ROWS - pad;
+      const int x0 = c * ROWS - pad;
       char* at = tiles + (c & 1) * kBuf;
-      TK::slow(at, kh + sp.base * R.k.st, sign * R.k.st, x0, kd);
-      TV::slow(at + TK::BYTES, vh + sp.base * R.v.st, sign * R.v.st, x0, vd);
-      if constexpr (OUT) TK::slow(at + TK::BYTES + TV::BYTES, qh + sp.base * R.q.st, sign * R.q.st, x0, kd);
+      TK::slow(at, kh + (int64_t)sp.base * R.k.st, sign * R.k.st, x0, kd);
+      TV::slow(at + TK::BYTES, vh + (int64_t)sp.base * R.v.st, sign * R.v.st, x0, vd);
+      if constexpr (OUT) TK::slow(at + TK::BYTES + TV::BYTES, qh + (int64_t)sp.base * R.q.st, sign * R.q.st, x0, kd);
       __syncthreads();
     }
     asm volatile("" : "+v"(row_x), "+v"(kcol_x) :: "memory");   // operands' places are worked out anew, not kept
