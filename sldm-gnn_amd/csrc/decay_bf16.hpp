@@ -134,10 +134,19 @@ __device__ __forceinline__ void update(f16v (&S)[KT], const bf8v (&vf)[2], const
   }
 }
 
+// LDS of a workgroup's tiles, and the waves a SIMD that leaves (up to 4, and 3
+// where the state alone takes 64 registers).
+template <int KT, int NW, bool OUT>
+constexpr int tile_bytes() { return 2 * C * (row_bytes(KT) * (OUT ? 2 : 1) + row_bytes(NW)); }
+constexpr int waves_for(int lds, int kt, int nw) {
+  const int w = (160 * 1024 / (lds + 512)) * nw / 4, most = kt == 4 ? 3 : 4;
+  return w < 1 ? 1 : w > most ? most : w;
+}
+
 // OUT: outputs, else the state alone.  EXACT: the roundings of a short sequence or
 // an output state (above).  FAST: by DMA, else by Tile::slow.
 template <int KT, int NW, bool OUT, bool EXACT, bool FAST>
-__global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_bf16_kernel(Args a) {
+__global__ __launch_bounds__(64 * NW, waves_for(tile_bytes<KT, NW, OUT>(), KT, NW)) void decay_bf16_kernel(Args a) {
   using TK = Tile<uint16_t, C, row_bytes(KT), NW, Swizzle>;
   using TV = Tile<uint16_t, C, row_bytes(NW), NW, Swizzle>;
   constexpr int NTH = 64 * NW, RBK = TK::kRB, RBV = TV::kRB;
