@@ -92,15 +92,23 @@ __global__ __launch_bounds__(256) void scan_kernel(float* loc, const float* s0, 
   if (s1) s1[bh * elems + e] = run;
 }
 
-// out[b, t, hk, :] = sum over the group's heads of part[b, t, hk * group + g, :]
+// out[b, t, hk, :] = sum over the group's heads of part[b, t, hk * group + g, :],
+// for dk (blockIdx.y 0) and dv (1)
+struct SumArgs {
+  const float* part[2];
+  void* out[2];
+  int64_t heads;   // B T Hk
+  int group, d[2];
+};
 template <typename T>
-__global__ __launch_bounds__(256) void sum_heads_kernel(const float* part, T* out, int64_t n, int group,
-                                                        int d) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+__global__ __launch_bounds__(256) void sum_heads_kernel(SumArgs a) {
+  const int w = blockIdx.y, d = a.d[w];
+  T* out = reinterpret_cast<T*>(a.out[w]);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.heads * d; i += (int64_t)gridDim.x * 256) {
     const int64_t head = i / d;
-    const float* p = part + head * group * d + i % d;
+    const float* p = a.part[w] + head * a.group * d + i % d;
     float s = p[0];
-    for (int g = 1; g < group; ++g) s += p[(int64_t)g * d];
+    for (int g = 1; g < a.group; ++g) s += p[(int64_t)g * d];
     if constexpr (sizeof(T) == 4) out[i] = s;
     else out[i] = sldm::f32_to_bf16(s);
   }
@@ -226,7 +234,7 @@ int check_shape(int dtype, int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t 
   SLDM_REQUIRE(dk >= 1 && dk <= kMaxDim && dv >= 1 && dv <= kMaxDim,
                "decay attention: head sizes must be in [1, %d], got %lld and %lld", kMaxDim, (long long)dk,
                (long long)dv);
-  SLDM_REQUIRE(B * H < kMaxThreads / 256 / 3, "decay attention: too many (batch, head) pairs: %lld",
+  SLDM_REQUIRE(B * H < kMaxThreads / 256 / 4, "decay attention: too many (batch, head) pairs: %lld",
                (long long)(B * H));
   return SLDM_OK;
 }
@@ -392,19 +400,14 @@ extern "C" int sldm_decay_attention_bwd(int dtype, const void* q, const int64_t*
   if (dv_out) roles[n++] = &rv;
   launch_roles(dtype, a, roles, n, true, st);
   SLDM_LAUNCH_CHECK("decay_kernel");
-  if (group > 1 && T > 0) {
-    for (int i = 0; i < 2; ++i) {
-      void* out = i ? dv_out : dk_out;
-      if (!out) continue;
-      const int d = (int)(i ? dv : dk);
-      const int64_t cnt = B * T * Hk * d;
-      const unsigned grid = (unsigned)std::min<int64_t>((cnt + 255) / 256, 1 << 16);
-      if (dtype == SLDM_F32)
-        sum_heads_kernel<float><<<grid, 256, 0, st>>>(i ? part_v : part_k, (float*)out, cnt, group, d);
-      else
-        sum_heads_kernel<uint16_t><<<grid, 256, 0, st>>>(i ? part_v : part_k, (uint16_t*)out, cnt, group, d);
-      SLDM_LAUNCH_CHECK("decay sum_heads_kernel");
-    }
+  if (group > 1 && T > 0 && (dk_out || dv_out)) {
+    SumArgs s{{part_k, part_v}, {dk_out, dv_out}, B * T * Hk, group, {(int)dk, (int)dv}};
+    if (!dk_out) s.part[0] = part_v, s.out[0] = dv_out, s.d[0] = (int)dv;
+    const int64_t most = s.heads * std::max(s.d[0], s.d[1]);
+    const dim3 grid((unsigned)std::min<int64_t>((most + 255) / 256, 1 << 15), dk_out && dv_out ? 2 : 1);
+    if (dtype == SLDM_F32) sum_heads_kernel<float><<<grid, 256, 0, st>>>(s);
+    else sum_heads_kernel<uint16_t><<<grid, 256, 0, st>>>(s);
+    SLDM_LAUNCH_CHECK("decay sum_heads_kernel");
   }
   return SLDM_OK;
 }

@@ -314,7 +314,10 @@ Dims check_qkv(const Tensor& q, const Tensor& k, const Tensor& v, int64_t lead, 
 }
 struct Ld {
   int64_t s[3];
-  explicit Ld(const Tensor& t) : s{t.stride(0), t.stride(1), t.stride(2)} {}
+  // the stride of a dimension of one says nothing, and may be any number
+  explicit Ld(const Tensor& t) {
+    for (int i = 0; i < 3; ++i) s[i] = t.size(i) == 1 ? 0 : t.stride(i);
+  }
 };
 Dims dims_of(const Tensor& q, const Tensor& k, const Tensor& v) {
   return {q.size(0), q.size(1), q.size(2), k.size(2), q.size(3), v.size(3)};

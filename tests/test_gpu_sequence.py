@@ -353,6 +353,56 @@ def test_decay_attention_strides(dtype):
     assert torch.equal(d1, d2)
 
 
+def test_decay_attention_one_long_dimension_strides():
+    """Dimensions of one with strides that mean nothing; one token of a long cache; time-major tensors."""
+    from sldm_sage import decay_attention
+    g = _gen(21)
+    x = _randn(g, 3, 50, 5, 16, dtype=torch.bfloat16)
+    ld = _decays(1)
+    one = x[1:2, :, 2:3].as_strided((1, 50, 1, 16), (7, x.stride(1), 3, 1), x[1:2, :, 2:3].storage_offset())
+    a, b = decay_attention(one, one, one, ld), decay_attention(*(x[1:2, :, 2:3].contiguous(),) * 3, ld)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    tm = _randn(g, 60, 4, 2, 16)                                    # [T, B, H, D]
+    a = decay_attention(*(tm.transpose(0, 1),) * 3, _decays(2))
+    b = decay_attention(*(tm.transpose(0, 1).contiguous(),) * 3, _decays(2))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_decay_attention_offsets_beyond_32_bits(dtype):
+    """Sequences whose bytes lie beyond 2^32 of the tensor's start (an expanded view costs no such memory to
+    read, a token stride beyond the fast path's reach takes the slow one)."""
+    from sldm_sage import decay_attention
+    g = _gen(22)
+    n = (1 << 32) // torch.empty(0, dtype=dtype).element_size() + 4096
+    big = torch.zeros(n, dtype=dtype, device=DEV)
+    small = _randn(g, 1, 40, 2, 16, dtype=dtype)
+    ld = _decays(2)
+    want = decay_attention(small, small, small, ld)
+    far = big[-40 * 32:].view(1, 40, 2, 16)
+    far.copy_(small)
+    batch = big.as_strided((2, 40, 2, 16), (n - 40 * 32, 32, 16, 1))     # batch 1 is `far`
+    o, s = decay_attention(batch, batch, batch, ld)
+    assert torch.equal(o[1], want[0][0]) and torch.equal(s[1], want[1][0]) and not o[0].any()
+    step = (n - 32) // 39                                               # tokens far apart
+    step -= step % 8
+    wide = big.as_strided((1, 40, 2, 16), (0, step, 16, 1))
+    wide.copy_(small)
+    o, s = decay_attention(wide, wide, wide, ld)
+    (wo, ws), (mo, ms) = (ref.decay_attention(t, t, t, ld, 0.25) for t in (small, small.abs()))
+    _within(o, wo, _att_bounds(U[dtype], 40, wo, mo), "out")
+    _within(s, ws, _att_bounds(2.0 ** -24, 40, ws, ms), "state")
+
+
+def test_second_derivatives_are_refused():
+    from sldm_sage import decay_attention, layer_norm, rotary_axes, rotary_frequencies
+    x = torch.randn(2, 5, 2, 16, device=DEV, requires_grad=True)
+    pos, f = torch.zeros(2, 5, 1, device=DEV), rotary_frequencies((8,), device=DEV)
+    for y in (layer_norm(x), rotary_axes(x, None, pos, f, (8,))[0], decay_attention(x, x, x, _decays(2))[0]):
+        with pytest.raises(RuntimeError, match="cannot be differentiated"):
+            torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
 @pytest.mark.parametrize("T", [90, 1300])
 def test_decay_attention_single_gradients(T):
     """Each gradient alone, and with only one of the two outputs used, equals that of the whole."""

@@ -141,6 +141,10 @@ def test_c_entries_refuse_before_any_launch():
     assert lib.sldm_decay_attention_step(1, None, None, None, None, None, None, 1, 3, 2, 16, 16, None, 1.0, None,
                                          None, None) == 1
     assert b"3 heads over 2" in lib.sldm_last_error()
+    assert lib.sldm_decay_attention_states_bytes(1, 1 << 22, 100, 1, 1, 8, 8) == 0
+    assert b"too many" in lib.sldm_last_error()
+    assert lib.sldm_decay_attention_fwd(0, None, None, None, None, None, None, 1 << 20, 1, 8, 8, 8, 8, None, 1.0,
+                                        None, None, 0, None, None, None, 0, None) == 1
     # long axes need room for their segments' states
     assert lib.sldm_decay_attention_states_bytes(1, 1, 100000, 1, 1, 64, 64) > 64 * 64 * 4 * 8
     assert lib.sldm_decay_attention_bwd_workspace_bytes(1, 1, 100000, 1, 1, 64, 64) > 64 * 64 * 4 * 8
