@@ -286,7 +286,7 @@ extern "C" int sldm_decay_attention_fwd(int dtype, const void* q, const int64_t*
   r.v = operand(v, ld_v, group, esz);
   set_out(r, out, T, H, dv, false, esz);
   r.kd = (int)dk; r.vd = (int)dv;
-  r.s_k = dv; r.s_v = 1;
+  r.s_k = (int)dv; r.s_v = 1;
   r.read_scale = r.p_scale = scale;
   r.upd_scale = 1.f;
   const Role* one[1] = {&r};
@@ -350,18 +350,18 @@ extern "C" int sldm_decay_attention_bwd(int dtype, const void* q, const int64_t*
   Role rq{}, rk{}, rv{};
   rq.q = od; rq.k = ov; rq.v = ok;               // dq_t = scale S_t do_t
   rq.kd = (int)dv; rq.vd = (int)dk;
-  rq.s_k = 1; rq.s_v = dv;
+  rq.s_k = 1; rq.s_v = (int)dv;
   rq.read_scale = rq.p_scale = scale; rq.upd_scale = 1.f;
   set_out(rq, dq, T, H, dk, false, esz);
   rv.q = ok; rv.k = oq; rv.v = od;               // dv_t = k_t G_t
   rv.kd = (int)dk; rv.vd = (int)dv;
-  rv.s_k = dv; rv.s_v = 1;
+  rv.s_k = (int)dv; rv.s_v = 1;
   rv.read_scale = 1.f; rv.p_scale = rv.upd_scale = scale;
   rv.delta = rv.reverse = 1;
   set_out(rv, group > 1 ? (void*)part_v : dv_out, T, H, dv, group > 1, esz);
   rk.q = ov; rk.k = od; rk.v = oq;               // dk_t = G_t v_t
   rk.kd = (int)dv; rk.vd = (int)dk;
-  rk.s_k = 1; rk.s_v = dv;
+  rk.s_k = 1; rk.s_v = (int)dv;
   rk.read_scale = 1.f; rk.p_scale = rk.upd_scale = scale;
   rk.delta = rk.reverse = 1;
   set_out(rk, group > 1 ? (void*)part_k : dk_out, T, H, dk, group > 1, esz);

@@ -48,7 +48,7 @@ struct Role {
   const float* s0;      // state before each segment (null: zero); element (a, c) at a s_k + c s_v
   float* s1;            // state behind each segment (null: not written), the same layout
   int64_t s0_bh, s0_seg, s1_bh, s1_seg;
-  int64_t s_k, s_v;
+  int s_k, s_v;
   float read_scale, p_scale, upd_scale;
   int delta, reverse;
   int kd, vd;
@@ -104,6 +104,32 @@ __device__ __forceinline__ Span span_of(const Args& a, const Role& R, int id) {
   s.base = R.reverse ? s.len - 1 - s.seg0 : s.seg0;
   s.ld2 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(a.log_decay[s.hd]))) * 1.44269504088896340736f;
   return s;
+}
+
+// The walk's state in memory: element (row, column) of a kd x vd state lies at
+// row s_k + column s_v.  N registers a lane, register i at row row_of(i); elements
+// outside the state are zeros.
+template <int N, typename RowOf>
+__device__ __forceinline__ void load_state(const Role& R, const float* s0, int col, bool whole, RowOf row_of, float (&v)[N]) {
+  if (whole) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = s0[row_of(i) * R.s_k + col * R.s_v];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = row_of(i);
+      v[i] = 0.f;
+      if (r < R.kd && col < R.vd) v[i] = s0[r * R.s_k + col * R.s_v];
+    }
+  }
+}
+template <int N, typename RowOf>
+__device__ __forceinline__ void store_state(const Role& R, float* s1, int col, bool whole, RowOf row_of, const float (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int r = row_of(i);
+    if (whole || (r < R.kd && col < R.vd)) s1[r * R.s_k + col * R.s_v] = v[i];
+  }
 }
 
 typedef __attribute__((address_space(3))) void* lds_vptr;

@@ -195,15 +195,16 @@ __global__ __launch_bounds__(64 * NW, waves_for(tile_bytes<KT, NW, OUT>(), KT, N
   for (int t = 0; t < KT; ++t)
 #pragma unroll
     for (int r = 0; r < 16; ++r) S[t][r] = 0.f;
+  const bool whole = kd == 32 * KT && vd == 32 * NW;
   if (R.s0) {
     const float* s0 = R.s0 + sp.bh * R.s0_bh + seg * R.s0_seg;
 #pragma unroll
-    for (int t = 0; t < KT; ++t)
+    for (int t = 0; t < KT; ++t) {
+      float x[16];
+      load_state(R, s0, vc, whole, [&](int r) { return 32 * t + 16 * (r >> 3) + 8 * h + (r & 7); }, x);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int kr = 32 * t + 16 * (r >> 3) + 8 * h + (r & 7);
-        if (kr < kd && vc < vd) S[t][r] = s0[kr * R.s_k + vc * R.s_v];
-      }
+      for (int r = 0; r < 16; ++r) S[t][r] = x[r];
+    }
   }
   // wtab[j]: the weight with which row j enters the state; dtab[32 + i - j]: D
   for (int j = threadIdx.x; j < C; j += NTH) wtab[j] = powg(ld2, C - 1 - j + R.delta) * R.upd_scale;
@@ -336,12 +337,12 @@ __global__ __launch_bounds__(64 * NW, waves_for(tile_bytes<KT, NW, OUT>(), KT, N
   if (R.s1) {
     float* s1 = R.s1 + sp.bh * R.s1_bh + seg * R.s1_seg;
 #pragma unroll
-    for (int t = 0; t < KT; ++t)
+    for (int t = 0; t < KT; ++t) {
+      float x[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int kr = 32 * t + 16 * (r >> 3) + 8 * h + (r & 7);
-        if (kr < kd && vc < vd) s1[kr * R.s_k + vc * R.s_v] = S[t][r];
-      }
+      for (int r = 0; r < 16; ++r) x[r] = S[t][r];
+      store_state(R, s1, vc, whole, [&](int r) { return 32 * t + 16 * (r >> 3) + 8 * h + (r & 7); }, x);
+    }
   }
   if constexpr (OUT) zero_tail<NTH, FAST>(a, R, sp, R.o_f32 ? 4 : 2);
 }

@@ -84,17 +84,17 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_f32_kernel(Arg
   for (int t = 0; t < KT; ++t)
 #pragma unroll
     for (int v = 0; v < NV; ++v) S[t][v] = f4v{0.f, 0.f, 0.f, 0.f};
+  const bool whole = kd == 16 * KT && vd == 16 * NV * NW;
   if (R.s0) {
     const float* s0 = R.s0 + sp.bh * R.s0_bh + seg * R.s0_seg;
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int kr = 16 * t + 4 * h + r, vc = v0 + 16 * v + m;
-          if (kr < kd && vc < vd) S[t][v][r] = s0[kr * R.s_k + vc * R.s_v];
-        }
+      for (int v = 0; v < NV; ++v) {
+        float x[4];
+        load_state(R, s0, v0 + 16 * v + m, whole, [&](int r) { return 16 * t + 4 * h + r; }, x);
+        S[t][v] = f4v{x[0], x[1], x[2], x[3]};
+      }
   }
   float d[4], w[4];                                  // D (lane = i, registers = j), the update's weights
 #pragma unroll
@@ -229,12 +229,10 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_f32_kernel(Arg
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int kr = 16 * t + 4 * h + r, vc = v0 + 16 * v + m;
-          if (kr < kd && vc < vd) s1[kr * R.s_k + vc * R.s_v] = S[t][v][r];
-        }
+      for (int v = 0; v < NV; ++v) {
+        const float x[4] = {S[t][v][0], S[t][v][1], S[t][v][2], S[t][v][3]};
+        store_state(R, s1, v0 + 16 * v + m, whole, [&](int r) { return 16 * t + 4 * h + r; }, x);
+      }
   }
   if constexpr (OUT) zero_tail<NTH, FAST>(a, R, sp, 4);
 }
