@@ -18,6 +18,7 @@ namespace {
 constexpr int kBlock = 256;
 constexpr int kMaxAxes = 8;
 constexpr int kMaxDim = 1024;
+constexpr int kMaxBlock = 64;   // tokens of a workgroup
 
 typedef uint32_t u4a2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u4a4 __attribute__((ext_vector_type(4), aligned(4)));
@@ -79,6 +80,7 @@ __device__ __forceinline__ double position(const RotArgs& a, int64_t off) {
 template <typename T, int V, bool MIX>
 __global__ __launch_bounds__(kBlock) void rotary_kernel(RotArgs a) {
   extern __shared__ float2 turn[];               // [tokens][pairs]: cos, sin
+  __shared__ int64_t q_at[kMaxBlock], k_at[kMaxBlock];   // where the tokens' rows start
   const int64_t n0 = (int64_t)blockIdx.x * a.block;
   const int64_t all = a.B * a.T;
   const int here = (int)(all - n0 < a.block ? all - n0 : a.block);
@@ -95,24 +97,35 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(RotArgs a) {
     sincosf((float)r, &s, &c);
     turn[i] = make_float2(c, a.sign * s);
   }
+  for (int i = threadIdx.x; i < here; i += kBlock) {
+    const int64_t b = (n0 + i) / a.T, t = (n0 + i) % a.T;
+    q_at[i] = b * a.q_sb + t * a.q_st;
+    k_at[i] = b * a.k_sb + t * a.k_st;
+  }
   __syncthreads();
-  const int rest = a.dim - 2 * a.pairs;
+  constexpr int F = 16 / (int)sizeof(T);
+  const int rest = a.dim - 2 * a.pairs;          // columns no axis turns: 16 bytes a lane where there are as many
   const int turned = MIX ? (2 * a.pairs + V - 1) / V : (a.pairs + V - 1) / V;
-  const int per = turned + (rest + V - 1) / V;   // pieces of a head
+  const int per = turned + (rest >= F ? (rest + F - 1) / F : rest);   // pieces of a head
   const int row = (a.hq + a.hk) * per;
   for (int i = threadIdx.x; i < here * row; i += kBlock) {
     const int tk = i / row, in_row = i % row;
     const int head = in_row / per, piece = in_row % per;
-    const int64_t n = n0 + tk, b = n / a.T, t = n % a.T;
     const bool is_q = head < a.hq;
     const int hd = is_q ? head : head - a.hq;
-    const T* src = reinterpret_cast<const T*>(is_q ? a.q : a.k) +
-                   (is_q ? b * a.q_sb + t * a.q_st + hd * a.q_sh : b * a.k_sb + t * a.k_st + hd * a.k_sh);
-    T* dst = reinterpret_cast<T*>(is_q ? a.oq : a.ok) + (n * (is_q ? a.hq : a.hk) + hd) * a.dim;
+    const T* src = reinterpret_cast<const T*>(is_q ? a.q : a.k) + (is_q ? q_at[tk] + hd * a.q_sh : k_at[tk] + hd * a.k_sh);
+    T* dst = reinterpret_cast<T*>(is_q ? a.oq : a.ok) + ((n0 + tk) * (is_q ? a.hq : a.hk) + hd) * a.dim;
     const float2* tr = turn + tk * a.pairs;
-    if (piece >= turned) {                       // columns no axis turns
-      const int c0 = 2 * a.pairs + (piece - turned) * V;
-      for (int e = 0; e < V && c0 + e < a.dim; ++e) dst[c0 + e] = src[c0 + e];
+    if (piece >= turned) {
+      if (rest >= F) {
+        const int c0 = min(2 * a.pairs + (piece - turned) * F, a.dim - F);
+        float x[F];
+        load_any<T, F>(src + c0, x);
+        store_any<T, F>(dst + c0, x);
+      } else {
+        const int c0 = 2 * a.pairs + piece - turned;
+        dst[c0] = src[c0];
+      }
     } else if constexpr (MIX) {
       // the last piece steps back to end with the last pair
       const int c0 = min(piece * V, 2 * a.pairs - V);
@@ -195,7 +208,7 @@ extern "C" int sldm_rotary_axes(int dtype, const void* q, const int64_t* ld_q, i
   a.freq = inv_freq;
   a.sign = inverse ? -1.f : 1.f;
   // about 512 angles a workgroup, fewer tokens while that leaves CUs idle
-  int64_t block = std::max<int64_t>(1, std::min<int64_t>(64, 512 / pairs));
+  int64_t block = std::max<int64_t>(1, std::min<int64_t>(kMaxBlock, 512 / pairs));
   block = std::max<int64_t>(1, std::min<int64_t>(block, B * T / 1024));
   const int64_t per_head = dim;   // an upper bound of a head's pieces
   SLDM_REQUIRE((heads_q + heads_k) * per_head * block < ((int64_t)1 << 31), "sldm_rotary_axes: too many heads");
