@@ -1,6 +1,6 @@
-// Host side of the decay attention operators (kernel: decay.hpp), the scan
-// that joins the segments of a long axis, the sum over shared heads, and the
-// single-token step.
+// Host side of the decay attention operators (mathematics: decay.hpp, kernels:
+// decay_f32.hip, decay_bf16.hpp), the scan that joins the segments of a long axis,
+// the sum over shared heads, and the single-token step.
 #include <algorithm>
 
 #include "decay.hpp"
@@ -18,7 +18,8 @@ constexpr int kChunk = 32;   // tokens of a segment are a multiple of this: no p
 // over k and v for the pieces' states, which are read and written too.  Fewer
 // than four pieces do not pay for that pass (bf16, 64 heads of 64, 1024 frames:
 // 59 us whole, 54 us in two, 40 in four; 128 heads, 512 frames: 34, 40, 37), nor
-// do short ones.  Waves aimed at, of 2048 / 3072 / 4096: bf16 (8 heads of 128,
+// do short ones, nor fewer than five in fp32 (1024 heads of 16, 2048 frames: 111 us
+// whole, 168 us in four).  Waves aimed at, of 2048 / 3072 / 4096: bf16 (8 heads of 128,
 // 32768 frames, training) 365 / 397 / 438 us, with 2048 for the forward alone 350 /
 // 334 / - us; fp32 (8 heads of 48 and 80, 1237 frames, training) 264 / 221 / 211 us.
 struct Plan {
@@ -31,6 +32,7 @@ Plan plan(int dtype, int64_t B, int64_t H, int64_t T, int64_t dk, int64_t dv, in
   const int64_t chunks = (T + C - 1) / C;
   const bool f32 = dtype == SLDM_F32;
   int64_t want = waves > 0 ? (f32 ? 4096 : roles == 3 ? 3072 : 2048) / waves : 1;
+  if (f32 && want < 5) want = 1;
   want = std::min(want, chunks / (f32 ? 4 : 8));
   if (want < 4) return {std::max<int64_t>(T, 1), 1};
   const int64_t per = (chunks + want - 1) / want;
