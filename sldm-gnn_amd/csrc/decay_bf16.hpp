@@ -12,6 +12,12 @@
 // spread over the banks.  Chunks of 64 (half as many state conversions) were
 // slower: their tiles and accumulators leave two waves a SIMD and spill.
 //
+// Measured (MI355X; copies 4.76 TB/s).  1024 heads, 2048 frames: 64-wide 228 us
+// (4.7 TB/s), 128-wide 503 us (4.3 TB/s), bound by memory; 16-wide 80 us (3.4
+// TB/s) and few long heads by the chain of a chunk (about 1 us from its first read
+// to its state).  8 heads of 128, 32768 frames: forward 41 us for the segments'
+// states, 14 for the scan, 59 for the outputs, backward 41, 14 and 160.
+//
 // Roundings.  The state is held in fp32 and read as bf16, and P = Q K^T o D is
 // rounded to bf16: the products of an output are each off by at most 2^-8 of
 // themselves, at random, and together by about what rounding the output costs
