@@ -144,6 +144,10 @@ class DecayEncoder(nn.Module):
         self.input_size, self.hidden_size, self.num_heads = input_size, hidden_size, num_heads
         self.head_dim = hidden_size // num_heads
         self.sections = [self.head_dim // 2] if sections is None else [int(n) for n in sections]
+        if not 1 <= len(self.sections) <= 8 or min(self.sections) < 0 or \
+                not 1 <= sum(self.sections) <= self.head_dim // 2:
+            raise ValueError(f"DecayEncoder: sections {self.sections} do not turn 1 to {self.head_dim // 2} pairs "
+                             "on 1 to 8 axes")
         fk = dict(device=device, dtype=dtype)
         self.norm = LayerNorm(hidden_size, **fk)
         self.embed = nn.Linear(input_size, hidden_size, **fk)
@@ -151,16 +155,22 @@ class DecayEncoder(nn.Module):
         self.head_norm = LayerNorm(self.head_dim, elementwise_affine=False)
         self.proj = nn.Linear(hidden_size, hidden_size, bias=False, **fk)
         # fading over 4 to 4 * 2^(heads - 1) frames, and the rotary ladder: fixed, and kept in
-        # their own types where the module's parameters are cast
-        self._log_decay = torch.log1p(-torch.exp2(-2.0 - torch.arange(num_heads, dtype=torch.float32)))
-        self._inv_freq = rotary_frequencies(self.sections, rotary_base)
+        # their own types where the module's parameters are cast (on the host whatever the default
+        # device, so that a module built on "meta" has them too)
+        heads = torch.arange(num_heads, dtype=torch.float32, device="cpu")
+        self._log_decay = torch.log1p(-torch.exp2(-2.0 - heads))
+        self._inv_freq = rotary_frequencies(self.sections, rotary_base, device="cpu")
         self._on: dict = {}
 
     def _tables(self, device: torch.device):
         t = self._on.get(device)
         if t is None:
-            t = self._on[device] = (self._log_decay.to(device), self._inv_freq.to(device))
+            with torch.inference_mode(False):      # kept: a later training pass saves them
+                t = self._on[device] = (self._log_decay.to(device), self._inv_freq.to(device))
         return t
+
+    def __getstate__(self):
+        return {**self.__dict__, "_on": {}}        # a copy's tables follow its own device
 
     def _qkv(self, x, positions):
         h = F.silu(self.embed(x))
@@ -199,6 +209,7 @@ class DecayEncoder(nn.Module):
         return self._out(h, o)
 
     def init_state(self, n: int, device=None):
-        """The state before the first frame of ``n`` sequences."""
-        return (torch.zeros(n, self.num_heads, self.head_dim, self.head_dim, device=device),
+        """The state before the first frame of ``n`` sequences (``device``: the parameters')."""
+        device = self.qkv.weight.device if device is None else device
+        return (torch.zeros(n, self.num_heads, self.head_dim, self.head_dim, dtype=torch.float32, device=device),
                 torch.zeros(n, dtype=torch.int64, device=device))

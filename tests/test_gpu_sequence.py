@@ -625,3 +625,20 @@ def test_decay_encoder_runs_like_the_gru():
         o, _ = ref.decay_attention(q, k, v, enc._log_decay.to(DEV), 0.25)
         want = h + ref.layer_norm(o).flatten(-2) @ d["proj.weight"].T
         torch.testing.assert_close(whole.double(), want, atol=1e-4, rtol=1e-4)
+
+
+def test_decay_encoder_served_before_it_is_trained():
+    """The first call under inference_mode leaves nothing behind that a training pass cannot save."""
+    from sldm_sage import DecayEncoder
+    torch.manual_seed(1)
+    enc = DecayEncoder(6, 64, num_heads=2).to(DEV)
+    x = torch.randn(3, 9, 6, device=DEV)
+    with torch.inference_mode():
+        served, _ = enc(x)
+        live = enc.init_state(3)
+        frames = torch.stack([enc.step(x[:, t], live) for t in range(9)], 1)
+        torch.testing.assert_close(frames, served, atol=1e-4, rtol=1e-4)
+    out, _ = enc(x)
+    assert torch.equal(out.detach(), served)
+    out.sum().backward()
+    assert all(p.grad is not None and p.grad.isfinite().all() for p in enc.parameters())

@@ -122,6 +122,31 @@ def test_encoder_refusals():
         sage.DecayEncoder(6, 9, num_heads=3)
     with pytest.raises(ValueError, match="expected"):
         sage.DecayEncoder(6, 96)(torch.zeros(2, 3, 7))
+    for sections in ((), (0, 0), (4, 5), (-1, 3)):
+        with pytest.raises(ValueError, match="sections"):
+            sage.DecayEncoder(6, 96, sections=sections)
+
+
+def test_encoder_tables_do_not_follow_the_default_device():
+    """A module built on "meta" (its parameters are filled later) still has its decays and frequencies, and a
+    pickled one leaves what it keeps for a device behind."""
+    import pickle
+    with torch.device("meta"):
+        enc = sage.DecayEncoder(6, 96, sections=(2, 3, 3))
+    like = sage.DecayEncoder(6, 96, sections=(2, 3, 3))
+    assert enc.qkv.weight.is_meta and enc.init_state(3)[0].is_meta
+    for a, b in zip(enc._tables(torch.device("cpu")), like._tables(torch.device("cpu"))):
+        assert torch.equal(a, b)
+    assert like._on and not pickle.loads(pickle.dumps(like))._on and like._on
+
+
+def test_encoder_tables_made_under_inference_mode_can_be_saved():
+    enc = sage.DecayEncoder(6, 96)
+    move = torch.Tensor.to
+    with torch.inference_mode(), pytest.MonkeyPatch.context() as patch:
+        patch.setattr(torch.Tensor, "to", lambda t, device: move(t, device, copy=True))
+        tables = enc._tables(torch.device("cpu"))
+    assert not any(t.is_inference() for t in tables)
 
 
 def test_c_entries_refuse_before_any_launch():
