@@ -484,14 +484,14 @@ void bwd(const T* x, int64_t ldx, const T* dy, int64_t lddy, int64_t rows, int64
                                                         rstd, dx, part)
     if (s.v == 1) SLDM_GO(1, 1, false);
     else if (s.wide) {
-      if (s.nch == 1) SLDM_GO(F, 1, true);
+      if (F == 8 && s.nch == 1) SLDM_GO(F, F == 8 ? 1 : 2, true);
       else if (s.nch == 2) SLDM_GO(F, 2, true);
       else if (s.nch <= 4) SLDM_GO(F, 4, true);
       else if constexpr (F == 4) SLDM_GO(F, 8, true);
     } else {
       if (s.nch == 1) SLDM_GO(F, 1, false);
       else if (s.nch == 2) SLDM_GO(F, 2, false);
-      else SLDM_GO(F, 4, false);
+      else if constexpr (F == 4) SLDM_GO(F, 4, false);
     }
 #undef SLDM_GO
   }
