@@ -11,6 +11,7 @@ namespace {
 constexpr int kMaxDim = 128;
 constexpr int64_t kMaxThreads = (int64_t)1 << 32;   // work-items of one launch, exclusive
 
+constexpr int kCUs = 256;
 constexpr int kChunk = 32;   // tokens of a segment are a multiple of this: no padding inside a sequence
 
 // Segments of the time axis.  One workgroup walks a sequence alone unless that
@@ -19,8 +20,8 @@ constexpr int kChunk = 32;   // tokens of a segment are a multiple of this: no p
 // than four pieces do not pay for that pass (bf16, 64 heads of 64, 1024 frames:
 // 59 us whole, 54 us in two, 40 in four; 128 heads, 512 frames: 34, 40, 37), nor
 // do short ones, nor fewer than five in fp32 (1024 heads of 16, 2048 frames: 111 us
-// whole, 168 us in four).  Waves aimed at, of 2048 / 3072 / 4096: bf16 (8 heads of 128,
-// 32768 frames, training) 365 / 397 / 438 us, with 2048 for the forward alone 350 /
+// whole, 168 us in four).  Waves aimed at, of 8 / 12 / 16 a CU: bf16 (8 heads of 128,
+// 32768 frames, training) 365 / 397 / 438 us, with 8 for the forward alone 350 /
 // 334 / - us; fp32 (8 heads of 48 and 80, 1237 frames, training) 264 / 221 / 211 us.
 struct Plan {
   int64_t seg_len;
@@ -31,7 +32,7 @@ Plan plan(int dtype, int64_t B, int64_t H, int64_t T, int64_t dk, int64_t dv, in
   const int64_t waves = B * H * roles * std::max(tiles_of((int)dk), tiles_of((int)dv));
   const int64_t chunks = (T + C - 1) / C;
   const bool f32 = dtype == SLDM_F32;
-  int64_t want = waves > 0 ? (f32 ? 4096 : roles == 3 ? 3072 : 2048) / waves : 1;
+  int64_t want = waves > 0 ? kCUs * (f32 ? 16 : roles == 3 ? 12 : 8) / waves : 1;
   if (f32 && want < 5) want = 1;
   want = std::min(want, chunks / (f32 ? 4 : 8));
   if (want < 4) return {std::max<int64_t>(T, 1), 1};

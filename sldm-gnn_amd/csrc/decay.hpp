@@ -207,6 +207,69 @@ __device__ __forceinline__ void zero_tail(const Args& a, const Role& R, const Sp
   }
 }
 
+// An infinity or NaN in a token's v would reach the outputs of the tokens in front of
+// it in the same chunk (as 0 times itself, in the masked half of P V), and in k
+// likewise.  It leaves a mark in the state that lasts to the end of the walk; a wave
+// that finds one there writes its columns' outputs anew by the recurrence itself,
+// token by token, where a token cannot reach what lies before it.  SPREAD: lanes
+// col + SPREAD, .. of the wave hold the other rows of a column.
+template <int N>
+__device__ __forceinline__ bool finite(const float (&v)[N]) {
+  float z = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) z = __builtin_fmaf(v[i], 0.f, z);
+  return z == 0.f;
+}
+// the lane's number, not kept in a register from the kernel's start
+__device__ __forceinline__ int lane_again() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t & 63;
+}
+__device__ __forceinline__ float widen(float v) { return v; }
+__device__ __forceinline__ float widen(uint16_t v) { return sldm::bf16_to_f32(v); }
+template <typename T, int N, int SPREAD, typename RowOf>
+__device__ __forceinline__ void walk_tokens(const Args& a, int order, int col, RowOf row_of) {
+  asm volatile("" : "+s"(order));                // the role is read anew, not kept over the walk before
+  const Role R = a.role[order % a.roles];
+  const Span s = span_of(a, R, order / a.roles);
+  const int seg = s.seg0 / (int)a.seg_len;
+  float S[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) S[i] = 0.f;
+  if (R.s0) load_state(R, R.s0 + s.bh * R.s0_bh + seg * R.s0_seg, col, false, row_of, S);
+  const T* q = reinterpret_cast<const T*>(R.q.p) + s.b * R.q.sb + (s.hd / R.q.hdiv) * R.q.sh;
+  const T* k = reinterpret_cast<const T*>(R.k.p) + s.b * R.k.sb + (s.hd / R.k.hdiv) * R.k.sh;
+  const T* v = reinterpret_cast<const T*>(R.v.p) + s.b * R.v.sb + (s.hd / R.v.hdiv) * R.v.sh;
+  const float g = exp2f(s.ld2), before = R.delta ? 1.f : g, after = R.delta ? g : 1.f;
+  // the chunks' outputs of this wave are in memory before these are
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll 1
+  for (int x = 0; x < s.n; ++x) {
+    const int64_t t = s.base + (R.reverse ? -x : x);
+    const float vv = col < R.vd ? widen(v[t * R.v.st + col]) * R.upd_scale : 0.f;
+    float o = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = row_of(i);
+      if (r < R.kd) {
+        S[i] = S[i] * before + widen(k[t * R.k.st + r]) * vv;
+        o += widen(q[t * R.q.st + r]) * S[i];
+        S[i] *= after;
+      }
+      if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int d = SPREAD; d < 64; d <<= 1) o += __shfl_xor(o, d);
+    o *= R.read_scale;
+    if (col < R.vd && (int)(threadIdx.x & 63) < SPREAD) {
+      const int64_t at = s.b * R.o_sb + t * R.o_st + s.hd * R.o_sh + col;
+      if (sizeof(T) == 4 || R.o_f32) reinterpret_cast<float*>(R.o)[at] = o;
+      else reinterpret_cast<uint16_t*>(R.o)[at] = sldm::f32_to_bf16(o);
+    }
+  }
+}
+
 // Rows of a chunk within 32-bit byte offsets of each other.
 inline bool near(const Operand& t) { return t.st >= 0 && t.st < ((int64_t)1 << 24); }
 // Whether every operand can come by DMA: rows on 16-byte boundaries, whole granules.

@@ -85,7 +85,8 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     float32 ``[B, H, Dk, Dv]`` is the state before the first token (None: zeros) and the returned
     one that behind the last.  ``lengths`` (int32 or int64 ``[B]``, clamped to ``[0, T]``): later
     tokens are padding, whatever they hold: outputs and gradients there are zeros and the state
-    ends before them.  Differentiable in q, k, v and state."""
+    ends before them.  An infinity or NaN reaches what these sums say and no token before its own.
+    Differentiable in q, k, v and state."""
     return _sldm()[2](q, k, v, log_decay, state, lengths, scale)
 
 

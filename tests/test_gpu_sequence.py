@@ -326,6 +326,43 @@ def test_decay_attention_long_axis(case, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("which", ["q", "k", "v", "do", "state"])
+@pytest.mark.parametrize("case", [(3, 70, 2, 1, 32, 48), (2, 45, 2, 2, 33, 7), (1, 1500, 1, 1, 64, 64), (2, 97, 4, 2, 128, 100),
+                                  (1, 700, 1, 1, 16, 16)], ids=str)
+def test_decay_attention_infinities_and_nan_stay_causal(case, which, dtype):
+    """One value that is not finite, in the middle of a chunk, reaches what the recurrences say and nothing else:
+    no output of an earlier token (of a later one, for the gradients of k and v), no other column of v."""
+    from sldm_sage import decay_attention
+    B, T, H, Hk, Dk, Dv = case
+    g = _gen(31)
+    t = {"q": _randn(g, B, T, H, Dk, dtype=dtype), "k": _randn(g, B, T, Hk, Dk, dtype=dtype),
+         "v": _randn(g, B, T, Hk, Dv, dtype=dtype), "do": _randn(g, B, T, H, Dv, dtype=dtype),
+         "state": _randn(g, B, H, Dk, Dv)}
+    dend, ld, scale = _randn(g, B, H, Dk, Dv), _decays(H), Dk ** -0.5
+    hit = t[which]
+    if which == "state":
+        hit[0, 0, Dk // 2, Dv // 3] = float("inf")
+    else:
+        hit[0, T // 2 + 3, 0, hit.size(3) // 2] = float("nan" if which in "qv" else "inf")
+        hit[0, T - 2, -1, 0] = -float("inf")
+    leaves = [t[n].clone().requires_grad_(True) for n in ("q", "k", "v", "state")]
+    o, end = decay_attention(*leaves[:3], ld, state=leaves[3])
+    grads = torch.autograd.grad((o, end), leaves, (t["do"], dend))
+    (wo, wend), wg = ref.decay_attention(t["q"], t["k"], t["v"], ld, scale, t["state"], None, t["do"], dend)
+    a = {n: x.abs() for n, x in t.items()}
+    (mo, mend), mg = ref.decay_attention(a["q"], a["k"], a["v"], ld, scale, a["state"], None, a["do"], dend.abs())
+    u, e = U[dtype], U[torch.float32]
+    some = False
+    for name, got, want, mag, uu in zip(("out", "state", "dq", "dk", "dv", "dstate"), (o, end, *grads), (wo, wend, *wg),
+                                        (mo, mend, *mg), (u, e, u, u, u, e)):
+        fine = want.isfinite()
+        some |= not fine.all()
+        assert torch.equal(got.isfinite(), fine), name
+        _within(got[fine], want[fine], _att_bounds(uu, T, want, mag)[fine], name)
+    assert some
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_decay_attention_strides(dtype):
     """Views of one projection, head-major tensors, expanded heads and gradients, columns not contiguous."""
     from sldm_sage import decay_attention
