@@ -19,7 +19,7 @@
 //
 // Measured (MI355X, where a copy of 1 GiB runs at 4.76 TB/s): 1M x 256 bf16
 // forward 218 us (4.7 TB/s), backward 307 us (5.0 TB/s) and 5 us for the sums;
-// 20011 x 1031 bf16 24, 45 and 4 us; 9600 x 96 fp32 4.6, 7.1 and 3.0 us, where
+// 20011 x 1031 bf16 20, 33 and 4 us; 9600 x 96 fp32 4.6, 7.1 and 3.0 us, where
 // the host's 68 us for the three launches and the autograd engine count.
 #include <algorithm>
 
@@ -405,8 +405,8 @@ __global__ __launch_bounds__(kSumCols* kSumRows) void norm_sum_kernel(const floa
 
 // Lanes and chunks of a row.  Up to 64 lanes x 4 chunks of 16 bytes a wave owns
 // it, then a workgroup up to 8192 elements; past that it is re-read.  The bf16
-// backward goes over to the workgroup at two chunks already: four hold 256
-// registers a lane (20011 x 2040: 64 us by waves, 54 us by workgroups).
+// backward goes over to the workgroup past three chunks: four hold 256 registers a
+// lane (20011 x 2040: 64 us by waves, 54 us by workgroups).
 struct Shape {
   int v, lpr_log2, nch;
   bool wide, loop;
@@ -423,6 +423,17 @@ Shape shape_of(int dtype, int64_t width, bool backward) {
   }
   const int64_t lpr = 1 << s.lpr_log2;
   while ((int64_t)s.nch * lpr < need) s.nch *= 2;
+  // bf16: three chunks where powers of two leave much room empty (forward / backward:
+  // 400000 x 264 112 -> 85 / 159 -> 133 us, 100000 x 513 51 -> 39 / 82 -> 72 us,
+  // 10000 x 4104 38 -> 30 / 87 -> 58 us; the backward at 500000 x 176, 22 of 32 chunks,
+  // would lose: 107 -> 114 us, and both at 1M x 96).  fp32 is at the memory's rate.
+  const int64_t room = s.nch * lpr, most = backward && room < 256 ? 5 : 6;   // eighths of it
+  if (full == 8 && !s.loop && room >= 32 && room != 512 && 8 * need <= most * room) {
+    s.nch = 3;
+    s.wide = room == 1024;
+    s.lpr_log2 = 0;
+    while ((int64_t)4 << s.lpr_log2 < room) ++s.lpr_log2;
+  }
   return s;
 }
 int64_t row_groups(const Shape& s, int64_t rows) {
@@ -455,12 +466,14 @@ void fwd(const T* x, int64_t ldx, int64_t rows, int64_t width, const float* w, c
   norm_fwd_kernel<T, V, N, W><<<grid, kBlock, 0, st>>>(x, ldx, rows, (int)width, s.lpr_log2, w, b, eps, y, mean, rstd)
   if (s.v == 1) SLDM_GO(1, 1, false);
   else if (s.wide) {
-    if (s.nch <= 2) SLDM_GO(F, 2, true);
-    else if (s.nch <= 4) SLDM_GO(F, 4, true);
+    if (s.nch == 2) SLDM_GO(F, 2, true);
+    else if (F == 8 && s.nch == 3) SLDM_GO(F, F == 8 ? 3 : 2, true);
+    else if (s.nch == 4) SLDM_GO(F, 4, true);
     else if constexpr (F == 4) SLDM_GO(F, 8, true);
   } else {
     if (s.nch == 1) SLDM_GO(F, 1, false);
     else if (s.nch == 2) SLDM_GO(F, 2, false);
+    else if (F == 8 && s.nch == 3) SLDM_GO(F, F == 8 ? 3 : 2, false);
     else SLDM_GO(F, 4, false);
   }
 #undef SLDM_GO
@@ -486,12 +499,13 @@ void bwd(const T* x, int64_t ldx, const T* dy, int64_t lddy, int64_t rows, int64
     else if (s.wide) {
       if (F == 8 && s.nch == 1) SLDM_GO(F, F == 8 ? 1 : 2, true);
       else if (s.nch == 2) SLDM_GO(F, 2, true);
-      else if (s.nch <= 4) SLDM_GO(F, 4, true);
+      else if (F == 8 && s.nch == 3) SLDM_GO(F, F == 8 ? 3 : 2, true);
+      else if (s.nch == 4) SLDM_GO(F, 4, true);
       else if constexpr (F == 4) SLDM_GO(F, 8, true);
     } else {
       if (s.nch == 1) SLDM_GO(F, 1, false);
       else if (s.nch == 2) SLDM_GO(F, 2, false);
-      else if constexpr (F == 4) SLDM_GO(F, 4, false);
+      else SLDM_GO(F, F == 8 ? 3 : 4, false);
     }
 #undef SLDM_GO
   }

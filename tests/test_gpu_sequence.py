@@ -68,7 +68,8 @@ def _norm_bounds(x, w, b, dy, eps):
 
 
 NORM_SHAPES = [(1, 1), (3, 5), (7, 8), (5, 17), (64, 96), (33, 100), (2, 3, 4, 16), (257, 256), (9, 1031), (130, 520),
-               (6, 2049), (3, 4098), (5, 8192), (4, 8193), (0, 64), (2, 20000), (5000, 24)]
+               (6, 2049), (3, 4098), (5, 8192), (4, 8193), (0, 64), (2, 20000), (5000, 24),
+               (70, 264), (300, 257), (41, 5000), (3, 6144), (600, 320), (23, 1536)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
