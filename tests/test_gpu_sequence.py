@@ -680,3 +680,102 @@ def test_decay_encoder_served_before_it_is_trained():
     assert torch.equal(out.detach(), served)
     out.sum().backward()
     assert all(p.grad is not None and p.grad.isfinite().all() for p in enc.parameters())
+
+
+def test_layer_norm_and_rotary_beyond_32_bits():
+    """More than 2^31 elements, and rows further apart than that: the last rows equal the same rows alone."""
+    from sldm_sage import layer_norm, rotary_axes, rotary_frequencies
+    w = torch.linspace(0.5, 1.5, 256, device=DEV)
+    x = torch.randn(8_400_000, 256, device=DEV, dtype=torch.bfloat16).requires_grad_(True)
+    assert x.numel() > 2 ** 31
+    y = layer_norm(x, w)
+    dx, = torch.autograd.grad(y, x, x.detach())
+    few = x.detach()[-1000:].clone().requires_grad_(True)
+    z = layer_norm(few, w)
+    assert torch.equal(y[-1000:], z)
+    assert torch.equal(dx[-1000:], torch.autograd.grad(z, few, few.detach())[0])
+    del y, dx, z
+    wide = x.detach().view(-1)[:2 ** 31].view(2, 2 ** 30)[:, -256:]
+    assert torch.equal(layer_norm(wide, w), layer_norm(wide.clone(), w))
+    del x, wide
+    T = 17_000_000
+    q = torch.randn(T, 2, 64, device=DEV, dtype=torch.bfloat16)
+    assert q.numel() > 2 ** 31
+    f, pos = rotary_frequencies((20, 12), device=DEV), torch.arange(T, device=DEV)[:, None].expand(T, 2)
+    out, _ = rotary_axes(q, None, pos, f, (20, 12))
+    assert torch.equal(out[-1000:], rotary_axes(q[-1000:], None, pos[-1000:], f, (20, 12))[0])
+
+
+def test_sequence_ops_from_two_host_threads():
+    """Two threads, each on a stream of its own, at once: the results of one after the other."""
+    import threading
+    from sldm_sage import decay_attention, layer_norm, rotary_axes, rotary_frequencies
+    g = _gen(41)
+    f, ld = rotary_frequencies((8, 8), device=DEV), _decays(4)
+    data = [(_randn(g, 2, t, 4, 32), torch.randint(0, 900, (2, t, 2), generator=g).to(DEV)) for t in (1300, 77)]
+
+    def program(x, pos):
+        leaf = x.clone().requires_grad_(True)
+        h = layer_norm(leaf)
+        q, k = rotary_axes(h, h[:, :, :2], pos, f, (8, 8))
+        o, s = decay_attention(q, k, h[:, :, 2:], ld)
+        return (o, s, *torch.autograd.grad((o, s), leaf, (torch.ones_like(o), torch.ones_like(s))))
+    want = [program(*d) for d in data]
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    got[i] = program(*data[i])
+            stream.synchronize()
+        except Exception as e:      # reported below: a thread's own error would pass unseen
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_decay_encoder_under_capture():
+    """A sequence, and live frames that move the state on in place, recorded and replayed on new inputs."""
+    from sldm_sage import DecayEncoder
+    torch.manual_seed(3)
+    enc = DecayEncoder(6, 96, num_heads=6, sections=(2, 3, 3)).to(DEV).requires_grad_(False)
+    x, pos = torch.zeros(5, 40, 6, device=DEV), torch.zeros(5, 40, 3, device=DEV)
+    lens = torch.full((5,), 40, device=DEV)
+    live = enc.init_state(5)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        enc(x, positions=pos, lengths=lens)
+        enc.step(x[:, 0], live, pos[:, 0])
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    whole, one = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(whole):
+        out, (S, seen) = enc(x, positions=pos, lengths=lens)
+    with torch.cuda.graph(one):
+        frame = enc.step(x[:, 0], live, pos[:, 0])
+    for turn in range(3):
+        x.copy_(torch.randn(5, 40, 6, device=DEV))
+        pos.copy_(torch.randn(5, 40, 3, device=DEV) * 20)
+        lens.copy_(torch.tensor([40, 0, 3 + turn, 32, 33], device=DEV))
+        for t in live:
+            t.zero_()
+        whole.replay()
+        torch.cuda.synchronize()
+        want, (wS, wseen) = enc(x, positions=pos, lengths=lens)
+        assert torch.equal(out, want) and torch.equal(S, wS) and torch.equal(seen, wseen)
+        again = enc.init_state(5)
+        for _ in range(4):
+            one.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(frame, enc.step(x[:, 0], again, pos[:, 0]))
+        assert torch.equal(live[0], again[0]) and torch.equal(live[1], again[1])
