@@ -184,8 +184,8 @@ __global__ __launch_bounds__(NTH) void step_kernel(StepArgs a) {
   }
 }
 
-Operand operand(const void* p, const int64_t* ld, int hdiv, int esz) {
-  Operand t{p, ld[0], ld[1], ld[2], hdiv, 1};
+Operand operand(const void* p, const int64_t* ld, bool shared, int esz) {
+  Operand t{p, ld[0], ld[1], ld[2], shared, 1};
   for (int i = 0; i < 3; ++i) t.vec &= (ld[i] * esz) % 16 == 0;
   t.vec &= reinterpret_cast<uintptr_t>(p) % 16 == 0;
   return t;
@@ -216,6 +216,12 @@ void launch_roles(int dtype, Args& a, const Role* const* roles, int n, bool out,
     // heads whose rows share 256 bytes
     const int64_t row = std::max<int64_t>(1, std::min(a.role[0].kd, a.role[0].vd)) * (dtype == SLDM_F32 ? 4 : 2);
     a.unit = m * (int)std::max<int64_t>(1, std::min<int64_t>(a.H, 256 / row));
+    a.hpw = 1;
+    a.by_unit = Div(a.unit);
+    a.by_roles = Div(m);
+    a.by_all = Div(a.B * a.H);
+    a.by_h = Div(a.H);
+    a.by_group = Div(a.group);
     if (dtype == SLDM_F32) run_f32(a, out, st);
     else run_bf16(a, out, st);
   }
@@ -281,13 +287,13 @@ extern "C" int sldm_decay_attention_fwd(int dtype, const void* q, const int64_t*
   const int64_t elems = dk * dv;
   hipStream_t st = sldm::as_stream(stream);
   Args a{};
-  a.B = B; a.H = H; a.T = T;
+  a.B = B; a.H = H; a.T = T; a.group = group;
   a.seg_len = p.seg_len; a.nseg = p.nseg; a.groups = (int)(B * H * p.nseg);
   a.log_decay = log_decay; a.lengths = lengths; a.lengths64 = lengths_int64;
   Role r{};
-  r.q = operand(q, ld_q, 1, esz);
-  r.k = operand(k, ld_k, group, esz);
-  r.v = operand(v, ld_v, group, esz);
+  r.q = operand(q, ld_q, false, esz);
+  r.k = operand(k, ld_k, group > 1, esz);
+  r.v = operand(v, ld_v, group > 1, esz);
   set_out(r, out, T, H, dv, false, esz);
   r.kd = (int)dk; r.vd = (int)dv;
   r.s_k = (int)dv; r.s_v = 1;
@@ -333,7 +339,7 @@ extern "C" int sldm_decay_attention_bwd(int dtype, const void* q, const int64_t*
   const int64_t elems = dk * dv;
   hipStream_t st = sldm::as_stream(stream);
   Args a{};
-  a.B = B; a.H = H; a.T = T;
+  a.B = B; a.H = H; a.T = T; a.group = group;
   a.log_decay = log_decay; a.lengths = lengths; a.lengths64 = lengths_int64;
   auto segments = [&](const Plan& s) {
     a.seg_len = s.seg_len; a.nseg = s.nseg; a.groups = (int)(B * H * s.nseg);
@@ -348,8 +354,8 @@ extern "C" int sldm_decay_attention_bwd(int dtype, const void* q, const int64_t*
     part_k = ws; ws += B * T * H * dk;
     part_v = ws;
   }
-  const Operand oq = operand(q, ld_q, 1, esz), ok = operand(k, ld_k, group, esz),
-                ov = operand(v, ld_v, group, esz), od = operand(dout, ld_do, 1, esz);
+  const Operand oq = operand(q, ld_q, false, esz), ok = operand(k, ld_k, group > 1, esz),
+                ov = operand(v, ld_v, group > 1, esz), od = operand(dout, ld_do, false, esz);
 
   Role rq{}, rk{}, rv{};
   rq.q = od; rq.k = ov; rq.v = ok;               // dq_t = scale S_t do_t

@@ -33,10 +33,30 @@
 
 namespace sldm_decay {
 
+// Division of 0 <= n < 2^31 by a divisor that the launch knows: the upper half of a
+// product, in scalar registers, instead of some thirty instructions.  With 2^s the
+// power of two from d on, n / d = (n + (n m >> 32)) >> s for m = floor(2^32 (2^s - d) / d) + 1.
+struct Div {
+  uint32_t d, m;
+  int s;
+  Div() = default;
+  explicit Div(int64_t by) : d((uint32_t)by), s(0) {
+    while (((int64_t)1 << s) < by) ++s;
+    m = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << s) - by)) / by + 1);
+  }
+  __device__ __forceinline__ int quotient(int n) const { return (int)((__umulhi((uint32_t)n, m) + (uint32_t)n) >> s); }
+  // n becomes the remainder
+  __device__ __forceinline__ int split(int& n) const {
+    const int q = quotient(n);
+    n -= q * (int)d;
+    return q;
+  }
+};
+
 struct Operand {
   const void* p;
   int64_t sb, st, sh;   // element strides of batch, token, head; columns are contiguous
-  int hdiv;             // head h reads head h / hdiv
+  int shared;           // head h reads head h / group
   int vec;              // every row starts on a 16-byte boundary
 };
 
@@ -57,8 +77,11 @@ struct Role {
 struct Args {
   Role role[3];
   int64_t B, H, T, seg_len;
-  int nseg, groups;     // groups = B H nseg
+  int nseg, groups;     // groups = B H nseg / hpw
+  int hpw;              // heads a workgroup has
   int roles, unit;      // unit: workgroups that stay together on an XCD
+  int group;            // heads that share a key head
+  Div by_unit, by_roles, by_all, by_h, by_group;   // by_all, by_h: B H / hpw, H / hpw
   const float* log_decay;
   const void* lengths;  // null: T each
   int lengths64;
@@ -78,32 +101,38 @@ __device__ __forceinline__ int64_t seq_len(const Args& a, int64_t b) {
 // tensors, and narrow heads share cache lines.  The units themselves go round the
 // XCDs, one place further each time, so that batches of uneven lengths do not
 // load some XCDs alone (ragged prompts: whole ranges of units an XCD 105 us).
-__device__ __forceinline__ int xcd_order(int unit) {
-  const int slot = (int)blockIdx.x >> 3, turn = slot / unit;
-  return (turn * 8 + (((int)blockIdx.x + turn) & 7)) * unit + slot % unit;
+__device__ __forceinline__ int xcd_order(const Args& a) {
+  int slot = (int)blockIdx.x >> 3;
+  const int turn = a.by_unit.split(slot);
+  return (turn * 8 + (((int)blockIdx.x + turn) & 7)) * a.unit + slot;
 }
 
 // What a (batch, head, segment) is made of.  All uniform, and said so: what comes
 // from a vector load would otherwise live in vector registers.
 struct Span {
   int64_t bh, b;
-  int hd, len, seg0, n, base;   // n: the segment's tokens; base: position x is token base +- x
+  int hd, len, seg, seg0, n, base;   // n: the segment's tokens; base: position x is token base +- x
   float ld2;                    // log2 of the decay
 };
-__device__ __forceinline__ Span span_of(const Args& a, const Role& R, int id) {
+// which: of the workgroup's heads.
+__device__ __forceinline__ Span span_of(const Args& a, const Role& R, int id, int which = 0) {
   Span s;
-  const int per = a.groups / a.nseg;
-  const int seg = id / per, H = (int)a.H;
-  s.bh = id % per;
-  s.b = (int)s.bh / H;
-  s.hd = (int)s.bh % H;
+  s.seg = a.by_all.split(id);
+  s.b = a.by_h.split(id);
+  s.hd = id * a.hpw + which;
+  s.bh = s.b * a.H + s.hd;
   s.len = __builtin_amdgcn_readfirstlane((int)seq_len(a, s.b));
-  s.seg0 = seg * (int)a.seg_len;
+  s.seg0 = s.seg * (int)a.seg_len;
   const int left = s.len - s.seg0, whole = (int)a.seg_len;
   s.n = left < 0 ? 0 : (left < whole ? left : whole);
   s.base = R.reverse ? s.len - 1 - s.seg0 : s.seg0;
   s.ld2 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(a.log_decay[s.hd]))) * 1.44269504088896340736f;
   return s;
+}
+
+template <typename T>
+__device__ __forceinline__ const T* head_of(const Args& a, const Operand& t, int64_t b, int hd) {
+  return reinterpret_cast<const T*>(t.p) + b * t.sb + (t.shared ? a.by_group.quotient(hd) : hd) * t.sh;
 }
 
 // The walk's state in memory: element (row, column) of a kd x vd state lies at
@@ -188,16 +217,16 @@ struct Tile {
 };
 
 // Tokens behind the sequence's end (of this segment's range): zeros, 16 bytes a
-// thread where the rows allow it.
+// thread where the rows allow it, by NTH threads (64: each wave for its own head).
 template <int NTH, bool FAST>
 __device__ __forceinline__ void zero_tail(const Args& a, const Role& R, const Span& s, int elem_bytes) {
   const int T = (int)a.T, whole = (int)a.seg_len, t1 = T - s.seg0 > whole ? s.seg0 + whole : T;
   const int t0 = s.len > s.seg0 ? s.len : s.seg0;
   if (t0 >= t1) return;
   constexpr int kLanes = 32;                     // across a row (of at most 512 bytes: 32 granules)
-  const int col = (int)threadIdx.x % kLanes, bytes = R.vd * elem_bytes;
+  const int col = (int)threadIdx.x % kLanes, row0 = (int)threadIdx.x % NTH / kLanes, bytes = R.vd * elem_bytes;
   char* o = reinterpret_cast<char*>(R.o) + (s.b * R.o_sb + s.hd * R.o_sh) * elem_bytes;
-  for (int t = t0 + (int)threadIdx.x / kLanes; t < t1; t += NTH / kLanes) {
+  for (int t = t0 + row0; t < t1; t += NTH / kLanes) {
     char* row = o + (int64_t)t * R.o_st * elem_bytes;
     if (FAST) {
       if (16 * col < bytes) *reinterpret_cast<uint4*>(row + 16 * col) = make_uint4(0, 0, 0, 0);
@@ -229,18 +258,18 @@ __device__ __forceinline__ int lane_again() {
 __device__ __forceinline__ float widen(float v) { return v; }
 __device__ __forceinline__ float widen(uint16_t v) { return sldm::bf16_to_f32(v); }
 template <typename T, int N, int SPREAD, typename RowOf>
-__device__ __forceinline__ void walk_tokens(const Args& a, int order, int col, RowOf row_of) {
+__device__ __forceinline__ void walk_tokens(const Args& a, int order, int which, int col, RowOf row_of) {
   asm volatile("" : "+s"(order));                // the role is read anew, not kept over the walk before
-  const Role R = a.role[order % a.roles];
-  const Span s = span_of(a, R, order / a.roles);
-  const int seg = s.seg0 / (int)a.seg_len;
+  const int id = a.by_roles.split(order);
+  const Role R = a.role[order];
+  const Span s = span_of(a, R, id, which);
   float S[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) S[i] = 0.f;
-  if (R.s0) load_state(R, R.s0 + s.bh * R.s0_bh + seg * R.s0_seg, col, false, row_of, S);
-  const T* q = reinterpret_cast<const T*>(R.q.p) + s.b * R.q.sb + (s.hd / R.q.hdiv) * R.q.sh;
-  const T* k = reinterpret_cast<const T*>(R.k.p) + s.b * R.k.sb + (s.hd / R.k.hdiv) * R.k.sh;
-  const T* v = reinterpret_cast<const T*>(R.v.p) + s.b * R.v.sb + (s.hd / R.v.hdiv) * R.v.sh;
+  if (R.s0) load_state(R, R.s0 + s.bh * R.s0_bh + s.seg * R.s0_seg, col, false, row_of, S);
+  const T* q = head_of<T>(a, R.q, s.b, s.hd);
+  const T* k = head_of<T>(a, R.k, s.b, s.hd);
+  const T* v = head_of<T>(a, R.v, s.b, s.hd);
   const float g = exp2f(s.ld2), before = R.delta ? 1.f : g, after = R.delta ? g : 1.f;
   // the chunks' outputs of this wave are in memory before these are
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");

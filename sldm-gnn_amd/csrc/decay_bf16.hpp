@@ -160,20 +160,21 @@ __global__ __launch_bounds__(64 * NW, waves_for(tile_bytes<KT, NW, OUT>(), KT, N
   __shared__ __attribute__((aligned(1024))) char tiles[2 * kBuf];
   __shared__ __attribute__((aligned(16))) float wtab[C], dtab[2 * C];
 
-  const int order = xcd_order(a.unit), id = order / a.roles;
+  const int order = xcd_order(a);
+  int role = order;
+  const int id = a.by_roles.split(role);
   if (id >= a.groups) return;
-  const Role R = a.role[order % a.roles];
+  const Role R = a.role[role];
   const Span sp = span_of(a, R, id);
-  const int seg = sp.seg0 / (int)a.seg_len;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 31, h = lane >> 5;
   const int kd = R.kd, vd = R.vd;
-  const int pad = (C - sp.n % C) % C, nch = (sp.n + pad) / C, sign = R.reverse ? -1 : 1;
+  const int pad = -sp.n & (C - 1), nch = (sp.n + pad) / C, sign = R.reverse ? -1 : 1;
   const float ld2 = sp.ld2;
 
-  const uint16_t* qh = OUT ? reinterpret_cast<const uint16_t*>(R.q.p) + sp.b * R.q.sb + (sp.hd / R.q.hdiv) * R.q.sh : nullptr;
-  const uint16_t* kh = reinterpret_cast<const uint16_t*>(R.k.p) + sp.b * R.k.sb + (sp.hd / R.k.hdiv) * R.k.sh;
-  const uint16_t* vh = reinterpret_cast<const uint16_t*>(R.v.p) + sp.b * R.v.sb + (sp.hd / R.v.hdiv) * R.v.sh;
+  const uint16_t* qh = OUT ? head_of<uint16_t>(a, R.q, sp.b, sp.hd) : nullptr;
+  const uint16_t* kh = head_of<uint16_t>(a, R.k, sp.b, sp.hd);
+  const uint16_t* vh = head_of<uint16_t>(a, R.v, sp.b, sp.hd);
 
   TK tq, tk;
   TV tv;
@@ -203,7 +204,7 @@ __global__ __launch_bounds__(64 * NW, waves_for(tile_bytes<KT, NW, OUT>(), KT, N
     for (int r = 0; r < 16; ++r) S[t][r] = 0.f;
   const bool whole = kd == 32 * KT && vd == 32 * NW;
   if (R.s0) {
-    const float* s0 = R.s0 + sp.bh * R.s0_bh + seg * R.s0_seg;
+    const float* s0 = R.s0 + sp.bh * R.s0_bh + sp.seg * R.s0_seg;
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
       float x[16];
@@ -341,7 +342,7 @@ __global__ __launch_bounds__(64 * NW, waves_for(tile_bytes<KT, NW, OUT>(), KT, N
   }
   if (OUT && nch > 0) put(nch - 1);
   if (R.s1) {
-    float* s1 = R.s1 + sp.bh * R.s1_bh + seg * R.s1_seg;
+    float* s1 = R.s1 + sp.bh * R.s1_bh + sp.seg * R.s1_seg;
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
       float x[16];
@@ -361,7 +362,7 @@ __global__ __launch_bounds__(64 * NW, waves_for(tile_bytes<KT, NW, OUT>(), KT, N
     }
     if (!__all(clean)) {
       const int l = lane_again();
-      walk_tokens<uint16_t, 16 * KT, 32>(a, order, 32 * wave + perm16(l & 31),
+      walk_tokens<uint16_t, 16 * KT, 32>(a, order, 0, 32 * wave + perm16(l & 31),
                                          [&](int i) { return 16 * (i >> 3) + 8 * (l >> 5) + (i & 7); });
     }
   }

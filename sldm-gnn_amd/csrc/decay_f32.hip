@@ -14,8 +14,8 @@
 // Measured (MI355X; copies 4.76 TB/s, an fp32 matrix product 153 TFLOP/s).  1024
 // heads, 2048 frames: 16-wide 112 us (4.8 TB/s) and 64-wide 490 us (4.4 TB/s),
 // bound by memory; 128-wide 1.49 ms, 121 TFLOP/s of issued products, bound by
-// them.  57600 heads of 16, 100 frames: forward 310 us (4.9 TB/s), backward 755 us
-// (3.4 TB/s of q, k, v, do, dq, dk, dv once each: short walks, three roles).
+// them.  57600 heads of 16, 100 frames: forward 290 us (5.1 TB/s), backward 610 us
+// (4.2 TB/s of q, k, v, do, dq, dk, dv once each).
 #include "decay.hpp"
 
 namespace sldm_decay {
@@ -39,29 +39,33 @@ struct Swizzle {
 };
 
 // KT: tiles of 16 state rows; NV: of 16 value columns a wave.  OUT: outputs, else
-// the state alone.  FAST: by DMA, else by Tile::slow.
-template <int KT, int NV, int NW, int SUB, bool OUT, bool FAST>
+// the state alone.  FAST: by DMA, else by Tile::slow.  PAIR: two waves have a head each,
+// neighbours whose rows lie side by side, and share the tiles.
+template <int KT, int NV, int NW, int SUB, bool OUT, bool FAST, bool PAIR>
 __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_f32_kernel(Args a) {
-  constexpr int RBK = KT == 6 ? 512 : 64 * KT, RBV = 64 * NV * NW, ROWS = C * SUB, NTH = 64 * NW;
+  static_assert(!PAIR || (KT == 1 && NV == 1 && NW == 2 && FAST), "pairs of narrow heads");
+  constexpr int HEADS = PAIR ? 2 : 1, RBK = KT == 6 ? 512 : 64 * KT * HEADS, RBV = 64 * NV * NW, ROWS = C * SUB, NTH = 64 * NW;
   using TK = Tile<float, ROWS, RBK, NW, Swizzle>;
   using TV = Tile<float, ROWS, RBV, NW, Swizzle>;
   constexpr int kBuf = TK::BYTES * (OUT ? 2 : 1) + TV::BYTES;       // k, v, q
   __shared__ __attribute__((aligned(1024))) char tiles[2 * kBuf];
 
-  const int order = xcd_order(a.unit), id = order / a.roles;
+  const int order = xcd_order(a);
+  int role = order;
+  const int id = a.by_roles.split(role);
   if (id >= a.groups) return;
-  const Role R = a.role[order % a.roles];
-  const Span sp = span_of(a, R, id);
-  const int seg = sp.seg0 / (int)a.seg_len;
+  const Role R = a.role[role];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), which = PAIR ? wave : 0;
+  const Span sp = span_of(a, R, id, which);
   const int lane = threadIdx.x & 63, m = lane & 15, h = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), v0 = 16 * NV * wave;
+  const int v0 = PAIR ? 0 : 16 * NV * wave;
   const int kd = R.kd, vd = R.vd;
-  const int pad = (ROWS - sp.n % ROWS) % ROWS, nt = (sp.n + pad) / ROWS, sign = R.reverse ? -1 : 1;
+  const int pad = -sp.n & (ROWS - 1), nt = (sp.n + pad) / ROWS, sign = R.reverse ? -1 : 1;
   const float ld2 = sp.ld2;
 
-  const float* qh = OUT ? reinterpret_cast<const float*>(R.q.p) + sp.b * R.q.sb + (sp.hd / R.q.hdiv) * R.q.sh : nullptr;
-  const float* kh = reinterpret_cast<const float*>(R.k.p) + sp.b * R.k.sb + (sp.hd / R.k.hdiv) * R.k.sh;
-  const float* vh = reinterpret_cast<const float*>(R.v.p) + sp.b * R.v.sb + (sp.hd / R.v.hdiv) * R.v.sh;
+  const float* qh = OUT ? head_of<float>(a, R.q, sp.b, sp.hd - which) : nullptr;
+  const float* kh = head_of<float>(a, R.k, sp.b, sp.hd - which);
+  const float* vh = head_of<float>(a, R.v, sp.b, sp.hd - which);
 
   TK tq, tk;
   TV tv;
@@ -73,13 +77,13 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_f32_kernel(Arg
     if constexpr (OUT) tq.load(c, at + TK::BYTES + TV::BYTES, first);
   };
   if (FAST && nt > 0) {
-    if (pad > 0 || kd * 4 < RBK || vd * 4 < RBV) {
+    if (pad > 0 || kd * HEADS * 4 < RBK || vd * HEADS * 4 < RBV) {
       for (int i = threadIdx.x; i < 2 * kBuf / 16; i += NTH) reinterpret_cast<uint4*>(tiles)[i] = make_uint4(0, 0, 0, 0);
       __syncthreads();
     }
-    tk.init(R.k, kh, sp, sign, pad, kd);
-    tv.init(R.v, vh, sp, sign, pad, vd);
-    if constexpr (OUT) tq.init(R.q, qh, sp, sign, pad, kd);
+    tk.init(R.k, kh, sp, sign, pad, kd * HEADS);
+    tv.init(R.v, vh, sp, sign, pad, vd * HEADS);
+    if constexpr (OUT) tq.init(R.q, qh, sp, sign, pad, kd * HEADS);
     fetch(0, pad);
   }
 
@@ -89,9 +93,9 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_f32_kernel(Arg
   for (int t = 0; t < KT; ++t)
 #pragma unroll
     for (int v = 0; v < NV; ++v) S[t][v] = f4v{0.f, 0.f, 0.f, 0.f};
-  const bool whole = kd == 16 * KT && vd == 16 * NV * NW;
+  const bool whole = kd == 16 * KT && vd == 16 * NV * NW / HEADS;
   if (R.s0) {
-    const float* s0 = R.s0 + sp.bh * R.s0_bh + seg * R.s0_seg;
+    const float* s0 = R.s0 + sp.bh * R.s0_bh + sp.seg * R.s0_seg;
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -113,7 +117,7 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_f32_kernel(Arg
   // where a lane finds granule h of row m, and column m of row 4 h; the swizzles are
   // XORs of bits, so other tiles and rows flip constant bits of the places
   const int row_at = m * RBK, kcol_at = 4 * h * RBK + 4 * (m & 3), vcol_at = 4 * h * RBV + 4 * (m & 3);
-  int row_x = (h ^ Swizzle<RBK>::of(m)) << 4, kcol_x = (m >> 2 ^ Swizzle<RBK>::of(4 * h)) << 4;
+  int row_x = (h ^ 4 * which ^ Swizzle<RBK>::of(m)) << 4, kcol_x = (m >> 2 ^ 4 * which ^ Swizzle<RBK>::of(4 * h)) << 4;
   const int vcol_x = (m >> 2 ^ Swizzle<RBV>::of(4 * h)) << 4;
   f4v O[SUB][NV];
   float* o_at = OUT ? reinterpret_cast<float*>(R.o) + sp.b * R.o_sb + (int64_t)(sp.base + sign * (m - pad)) * R.o_st +
@@ -230,7 +234,7 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_f32_kernel(Arg
   }
   if (OUT && nt > 0) put(nt - 1);
   if (R.s1) {
-    float* s1 = R.s1 + sp.bh * R.s1_bh + seg * R.s1_seg;
+    float* s1 = R.s1 + sp.bh * R.s1_bh + sp.seg * R.s1_seg;
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -252,16 +256,16 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_f32_kernel(Arg
       const int l = lane_again();
 #pragma unroll 1
       for (int v = 0; v < NV; ++v)
-        walk_tokens<float, 4 * KT, 16>(a, order, v0 + 16 * v + (l & 15),
+        walk_tokens<float, 4 * KT, 16>(a, order, which, v0 + 16 * v + (l & 15),
                                        [&](int i) { return 16 * (i >> 2) + 4 * (l >> 4) + (i & 3); });
     }
   }
-  if constexpr (OUT) zero_tail<NTH, FAST>(a, R, sp, 4);
+  if constexpr (OUT) zero_tail<PAIR ? 64 : NTH, FAST>(a, R, sp, 4);
 }
 
-template <int KT, int NV, int NW, int SUB, bool OUT, bool FAST = true>
+template <int KT, int NV, int NW, int SUB, bool OUT, bool FAST = true, bool PAIR = false>
 void launch(const Args& a, hipStream_t st) {
-  decay_f32_kernel<KT, NV, NW, SUB, OUT, FAST>
+  decay_f32_kernel<KT, NV, NW, SUB, OUT, FAST, PAIR>
       <<<grid_of(a), 64 * NW, 0, st>>>(a);
 }
 // Tiles of 32 tokens while a head is narrow, of 16 where 32 would leave a CU short
@@ -274,6 +278,18 @@ void by_cols(const Args& a, int vd, hipStream_t st) {
   else if (vd <= 64) launch<KT, 2, 2, 1, OUT>(a, st);
   else launch<KT, 2, 4, 1, OUT>(a, st);
 }
+// Pairs of 16-wide heads make rows of 128 bytes, a cache line: half lines bound the
+// backward, whose roles read them nine times (57600 heads, 100 frames: 738 us by single
+// heads, whatever the tiles in flight and the order of the products; 627 by pairs).
+bool pairs(const Args& a) {
+  bool ok = a.H % 2 == 0;
+  for (int i = 0; i < a.roles; ++i) {
+    const Role& r = a.role[i];
+    ok = ok && r.kd == 16 && r.vd == 16;
+    for (const Operand* t : {&r.q, &r.k, &r.v}) ok = ok && !t->shared && t->sh == 16;
+  }
+  return ok;
+}
 template <bool OUT>
 void run(const Args& a, hipStream_t st) {
   int kd = 0, vd = 0;
@@ -281,7 +297,18 @@ void run(const Args& a, hipStream_t st) {
     kd = a.role[i].kd > kd ? a.role[i].kd : kd;
     vd = a.role[i].vd > vd ? a.role[i].vd : vd;
   }
-  if (!all_fast(a, OUT, 4)) launch<8, 2, 4, 1, OUT, false>(a, st);
+  if (!all_fast(a, OUT, 4)) {
+    launch<8, 2, 4, 1, OUT, false>(a, st);
+  } else if (pairs(a)) {
+    Args two = a;
+    two.hpw = 2;
+    two.groups = a.groups / 2;
+    two.unit = a.roles * (a.H % 4 ? 1 : 2);
+    two.by_unit = Div(two.unit);
+    two.by_all = Div(a.B * a.H / 2);
+    two.by_h = Div(a.H / 2);
+    launch<1, 1, 2, 2, OUT, true, true>(two, st);
+  }
   else if (kd <= 16) by_cols<1, OUT>(a, vd, st);
   else if (kd <= 32) by_cols<2, OUT>(a, vd, st);
   else if (kd <= 64) by_cols<4, OUT>(a, vd, st);

@@ -298,12 +298,13 @@ def test_decay_attention_decay_extremes(kind, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("itype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("heads", [(2, 1, 32, 48), (6, 6, 16, 16)], ids=str)
 @pytest.mark.parametrize("T", [5, 70, 300, 700])
-def test_decay_attention_ragged(T, itype, dtype):
+def test_decay_attention_ragged(T, heads, itype, dtype):
     """Lengths 0, 1, at and around the chunks' ends, beyond T and below 0 (clamped); NaN and Inf behind them."""
     g = _gen(10)
     lens = torch.tensor([0, 1, T, T + 9, -3, min(T, 31), min(T, 64), min(T, 65), T - 1, T // 2], dtype=itype, device=DEV)
-    B, H, Hk, Dk, Dv = lens.numel(), 2, 1, 32, 48
+    B, (H, Hk, Dk, Dv) = lens.numel(), heads
     q, k, v = (_randn(g, B, T, h, d, dtype=dtype) for h, d in ((H, Dk), (Hk, Dk), (Hk, Dv)))
     do, dend, state = _randn(g, B, T, H, Dv, dtype=dtype), _randn(g, B, H, Dk, Dv), _randn(g, B, H, Dk, Dv)
     behind = ~(torch.arange(T, device=DEV) < lens[:, None])
@@ -314,7 +315,8 @@ def test_decay_attention_ragged(T, itype, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("case", [(1, 2500, 2, 1, 64, 64), (2, 1111, 1, 1, 128, 40), (1, 4100, 1, 1, 16, 16)], ids=str)
+@pytest.mark.parametrize("case", [(1, 2500, 2, 1, 64, 64), (2, 1111, 1, 1, 128, 40), (1, 4100, 1, 1, 16, 16),
+                                  (2, 2100, 4, 4, 16, 16)], ids=str)
 def test_decay_attention_long_axis(case, dtype):
     """Few heads and a long axis: the axis is cut into segments."""
     B, T, H, Hk, Dk, Dv = case
@@ -329,7 +331,7 @@ def test_decay_attention_long_axis(case, dtype):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("which", ["q", "k", "v", "do", "state"])
 @pytest.mark.parametrize("case", [(3, 70, 2, 1, 32, 48), (2, 45, 2, 2, 33, 7), (1, 1500, 1, 1, 64, 64), (2, 97, 4, 2, 128, 100),
-                                  (1, 700, 1, 1, 16, 16)], ids=str)
+                                  (1, 700, 1, 1, 16, 16), (2, 75, 4, 4, 16, 16)], ids=str)
 def test_decay_attention_infinities_and_nan_stay_causal(case, which, dtype):
     """One value that is not finite, in the middle of a chunk, reaches what the recurrences say and nothing else:
     no output of an earlier token (of a later one, for the gradients of k and v), no other column of v."""
