@@ -44,7 +44,8 @@ struct Swizzle {
 template <int KT, int NV, int NW, int SUB, bool OUT, bool FAST, bool PAIR>
 __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_f32_kernel(Args a) {
   static_assert(!PAIR || (KT == 1 && NV == 1 && NW == 2 && FAST), "pairs of narrow heads");
-  constexpr int HEADS = PAIR ? 2 : 1, RBK = KT == 6 ? 512 : 64 * KT * HEADS, RBV = 64 * NV * NW, ROWS = C * SUB, NTH = 64 * NW;
+  constexpr int HEADS = PAIR ? 2 : 1, ROWS = C * SUB, NTH = 64 * NW;
+  constexpr int RBK = KT > 4 ? 512 : KT == 3 ? 256 : 64 * KT * HEADS, RBV = (NW == 3 ? 4 : NW) * 64 * NV;   // powers of two
   using TK = Tile<float, ROWS, RBK, NW, Swizzle>;
   using TV = Tile<float, ROWS, RBV, NW, Swizzle>;
   constexpr int kBuf = TK::BYTES * (OUT ? 2 : 1) + TV::BYTES;       // k, v, q
@@ -270,12 +271,17 @@ void launch(const Args& a, hipStream_t st) {
 }
 // Tiles of 32 tokens while a head is narrow, of 16 where 32 would leave a CU short
 // of workgroups.
+// State rows in steps of 16 and value columns of 48 and 96 of their own: 9600 x 2
+// heads of 48, 100 frames, training 1740 us padded to 64, 1410 us like this; 8 heads
+// over 2 of 48 and 80, 5 x 1237 frames 154 and 125 us.
 template <int KT, bool OUT>
 void by_cols(const Args& a, int vd, hipStream_t st) {
   constexpr int SUB = KT == 1 ? 2 : 1;
   if (vd <= 16) launch<KT, 1, 1, SUB, OUT>(a, st);
   else if (vd <= 32) launch<KT, 2, 1, SUB, OUT>(a, st);
+  else if (vd <= 48) launch<KT, 1, 3, 1, OUT>(a, st);
   else if (vd <= 64) launch<KT, 2, 2, 1, OUT>(a, st);
+  else if (vd <= 96) launch<KT, 2, 3, 1, OUT>(a, st);
   else launch<KT, 2, 4, 1, OUT>(a, st);
 }
 // Pairs of 16-wide heads make rows of 128 bytes, a cache line: half lines bound the
@@ -311,7 +317,9 @@ void run(const Args& a, hipStream_t st) {
   }
   else if (kd <= 16) by_cols<1, OUT>(a, vd, st);
   else if (kd <= 32) by_cols<2, OUT>(a, vd, st);
+  else if (kd <= 48) by_cols<3, OUT>(a, vd, st);
   else if (kd <= 64) by_cols<4, OUT>(a, vd, st);
+  else if (kd <= 80) by_cols<5, OUT>(a, vd, st);
   else if (kd <= 96) by_cols<6, OUT>(a, vd, st);
   else by_cols<8, OUT>(a, vd, st);
 }
