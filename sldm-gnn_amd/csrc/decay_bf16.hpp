@@ -18,14 +18,13 @@
 // to its state).  8 heads of 128, 32768 frames: forward 41 us for the segments'
 // states, 14 for the scan, 59 for the outputs, backward 41, 14 and 160.
 //
-// Roundings.  The state is held in fp32 and read as bf16, and P = Q K^T o D is
-// rounded to bf16: the products of an output are each off by at most 2^-8 of
-// themselves, at random, and together by about what rounding the output costs
-// (relative error 0.0024 with both, 0.0017 for the rounding of the output alone).
-// The state's update takes V g^{n-1-j} as hi + mid (16 significant bits).  Where
-// the walk's state is an output, in fp32, it takes hi + mid + lo (all 24), and P
-// goes in as hi + lo; so in short sequences, whose outputs hang on few entries of
-// P, which do not average out.  (Both in one kernel, chosen by a branch, spill.)
+// Roundings.  The state is held in fp32 accumulators.  What the matrix instructions
+// take from fp32 goes in as sums of bf16 terms: the state that is read, and P = Q K^T
+// o D, as hi + lo (16 significant bits, so the products of an output are each off by
+// at most 2^-16 of themselves, far below what rounding the output to bf16 costs), and
+// V g^{n-1-j}, which enters the state, as hi + mid + lo (all 24).  One term for the
+// state or for P would be as large an error as the output's own rounding (relative
+// error 0.0024 instead of 0.0017), and more where the products cancel.
 #pragma once
 
 #include "decay.hpp"
@@ -38,18 +37,11 @@ typedef short s4v __attribute__((ext_vector_type(4)));
 typedef short s8v __attribute__((ext_vector_type(8)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 constexpr int C = 32;
-constexpr int kShort = 128;      // tokens of a sequence that counts as short
 
 __device__ __forceinline__ f16v mfma(bf8v a, bf8v b, f16v c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 __device__ __forceinline__ bf8v as_bf8(sldm::bf16x8 v) { return __builtin_bit_cast(bf8v, v); }
-__device__ __forceinline__ bf8v pack8(const float (&v)[8]) {
-  uint32_t w[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) w[e] = sldm::pack_bf16x2(v[2 * e], v[2 * e + 1]);
-  return __builtin_bit_cast(bf8v, make_uint4(w[0], w[1], w[2], w[3]));
-}
 
 // LDS rows of 32 DT values (96 take the room of 128); swizzle: granule g of row r
 // lies at g ^ swz(r).  Four neighbouring rows' transposed reads (64 bytes of
@@ -106,8 +98,8 @@ struct ColRead {
 // all products are in registers at once and spill.
 __device__ __forceinline__ void phase() { __builtin_amdgcn_sched_barrier(0); }
 
-// The state's update: S <- g^n S + K^T diag(w) V, V diag(w) in TERMS parts.
-template <int KT, int TERMS>
+// The state's update: S <- g^n S + K^T diag(w) V, V diag(w) in three parts.
+template <int KT>
 __device__ __forceinline__ void update(f16v (&S)[KT], const bf8v (&vf)[2], const char* lk, const ColRead& ck,
                                        const float* pw, float gn) {
   bf8v kf[2][KT];
@@ -121,8 +113,7 @@ __device__ __forceinline__ void update(f16v (&S)[KT], const bf8v (&vf)[2], const
                         sldm::bf16_hi(u.y) * w[3], sldm::bf16_lo(u.z) * w[4], sldm::bf16_hi(u.z) * w[5],
                         sldm::bf16_lo(u.w) * w[6], sldm::bf16_hi(u.w) * w[7]};
     sldm::bf16x8 hi, mid, lo;
-    if constexpr (TERMS == 3) sldm::split3_bf16x8(x, hi, mid, lo);
-    else sldm::split_bf16x8(x, hi, mid);
+    sldm::split3_bf16x8(x, hi, mid, lo);
     phase();
     if (s == 0)
 #pragma unroll
@@ -132,7 +123,7 @@ __device__ __forceinline__ void update(f16v (&S)[KT], const bf8v (&vf)[2], const
       if (s == 0)
 #pragma unroll
         for (int r = 0; r < 16; ++r) S[t][r] *= gn;
-      if constexpr (TERMS == 3) S[t] = mfma(kf[s][t], as_bf8(lo), S[t]);
+      S[t] = mfma(kf[s][t], as_bf8(lo), S[t]);
       S[t] = mfma(kf[s][t], as_bf8(mid), S[t]);
       S[t] = mfma(kf[s][t], as_bf8(hi), S[t]);
     }
@@ -149,9 +140,8 @@ constexpr int waves_for(int lds, int kt, int nw) {
   return w < 1 ? 1 : w > most ? most : w;
 }
 
-// OUT: outputs, else the state alone.  EXACT: the roundings of a short sequence or
-// an output state (above).  FAST: by DMA, else by Tile::slow.
-template <int KT, int NW, bool OUT, bool EXACT, bool FAST>
+// OUT: outputs, else the state alone.  FAST: by DMA, else by Tile::slow.
+template <int KT, int NW, bool OUT, bool FAST>
 __global__ __launch_bounds__(64 * NW, waves_for(tile_bytes<KT, NW, OUT>(), KT, NW)) void decay_bf16_kernel(Args a) {
   using TK = Tile<uint16_t, C, row_bytes(KT), NW, Swizzle>;
   using TV = Tile<uint16_t, C, row_bytes(NW), NW, Swizzle>;
@@ -315,8 +305,11 @@ __global__ __launch_bounds__(64 * NW, waves_for(tile_bytes<KT, NW, OUT>(), KT, N
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = S[t >> 1][8 * (t & 1) + e];
-        O = mfma(pack8(x), qf, O);
+        sldm::bf16x8 hi, lo;
+        sldm::split_bf16x8(x, hi, lo);
+        O = mfma(as_bf8(lo), qf, O);
         P = mfma(kf, qf, P);
+        O = mfma(as_bf8(hi), qf, O);
         phase();
       }
 #pragma unroll
@@ -326,17 +319,13 @@ __global__ __launch_bounds__(64 * NW, waves_for(tile_bytes<KT, NW, OUT>(), KT, N
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = P[8 * s + e] * pd[23 - 16 * s - e];
-        if constexpr (EXACT) {
-          sldm::bf16x8 hi, lo;
-          sldm::split_bf16x8(x, hi, lo);
-          O = mfma(vf[s], as_bf8(lo), O);
-          O = mfma(vf[s], as_bf8(hi), O);
-        } else {
-          O = mfma(vf[s], pack8(x), O);
-        }
+        sldm::bf16x8 hi, lo;
+        sldm::split_bf16x8(x, hi, lo);
+        O = mfma(vf[s], as_bf8(lo), O);
+        O = mfma(vf[s], as_bf8(hi), O);
       }
     }
-    update<KT, EXACT ? 3 : 2>(S, vf, lk, ck, pw, gn);
+    update<KT>(S, vf, lk, ck, pw, gn);
     rd = rd_full;
     gn = gn_full;
   }
@@ -369,24 +358,24 @@ __global__ __launch_bounds__(64 * NW, waves_for(tile_bytes<KT, NW, OUT>(), KT, N
   if constexpr (OUT) zero_tail<NTH, FAST>(a, R, sp, R.o_f32 ? 4 : 2);
 }
 
-template <int KT, int NW, bool OUT, bool EXACT, bool FAST = true>
+template <int KT, int NW, bool OUT, bool FAST = true>
 void launch(const Args& a, hipStream_t st) {
-  decay_bf16_kernel<KT, NW, OUT, EXACT, FAST>
+  decay_bf16_kernel<KT, NW, OUT, FAST>
       <<<grid_of(a), 64 * NW, 0, st>>>(a);
 }
-template <int KT, bool OUT, bool EXACT>
+template <int KT, bool OUT>
 void by_cols(const Args& a, int nw, hipStream_t st) {
-  if (nw == 1) launch<KT, 1, OUT, EXACT>(a, st);
-  else if (nw == 2) launch<KT, 2, OUT, EXACT>(a, st);
-  else launch<KT, 4, OUT, EXACT>(a, st);
+  if (nw == 1) launch<KT, 1, OUT>(a, st);
+  else if (nw == 2) launch<KT, 2, OUT>(a, st);
+  else launch<KT, 4, OUT>(a, st);
 }
-template <bool OUT, bool EXACT>
+template <bool OUT>
 void by_rows(const Args& a, hipStream_t st) {
   const int kt = row_tiles(a.role[0].kd), nw = tiles_of(a.role[0].vd);
-  if (kt == 1) by_cols<1, OUT, EXACT>(a, nw, st);
-  else if (kt == 2) by_cols<2, OUT, EXACT>(a, nw, st);
-  else if (kt == 3) by_cols<3, OUT, EXACT>(a, nw, st);
-  else by_cols<4, OUT, EXACT>(a, nw, st);
+  if (kt == 1) by_cols<1, OUT>(a, nw, st);
+  else if (kt == 2) by_cols<2, OUT>(a, nw, st);
+  else if (kt == 3) by_cols<3, OUT>(a, nw, st);
+  else by_cols<4, OUT>(a, nw, st);
 }
 }  // namespace
 }  // namespace sldm_decay
