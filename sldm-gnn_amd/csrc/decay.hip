@@ -57,7 +57,12 @@ Plans plans(int dtype, int64_t B, int64_t H, int64_t T, int64_t dk, int64_t dv) 
 }
 
 // loc[bh][s]: the states that segments add, each from zero -> the states
-// before each segment, and the state behind the last one.
+// before each segment, and the state behind the last one.  A segment's decay may be
+// zero in fp32 where a token's is not: it leaves an infinity one.
+__device__ __forceinline__ float faded(float s, float g, bool keeps) {
+  const float r = s * g;
+  return keeps && r != r ? s : r;
+}
 __global__ __launch_bounds__(256) void scan_kernel(float* loc, const float* s0, float* s1, Args a,
                                                    int64_t elems) {
   const int64_t bh = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
@@ -68,6 +73,7 @@ __global__ __launch_bounds__(256) void scan_kernel(float* loc, const float* s0, 
   float run = s0 ? s0[bh * elems + e] : 0.f;
   float* p = loc + bh * a.nseg * elems + e;
   const float g = exp2f(ld2 * (float)a.seg_len);
+  const bool keeps = exp2f(ld2) > 0.f;
   const int whole = (int)(len / a.seg_len);   // segments without padding
   int s = 0;
   for (; s + 8 <= whole; s += 8) {             // eight loads in flight
@@ -77,19 +83,19 @@ __global__ __launch_bounds__(256) void scan_kernel(float* loc, const float* s0, 
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       p[(s + i) * elems] = run;
-      run = run * g + add[i];
+      run = faded(run, g, keeps) + add[i];
     }
   }
   for (; s < whole; ++s) {
     const float add = p[s * elems];
     p[s * elems] = run;
-    run = run * g + add;
+    run = faded(run, g, keeps) + add;
   }
   if (s < a.nseg) {
     const int64_t n = len - (int64_t)s * a.seg_len;
     const float add = p[s * elems];
     p[s * elems] = run;
-    run = run * powg(ld2, (int)n) + add;
+    run = faded(run, powg(ld2, (int)n), keeps) + add;
     for (++s; s < a.nseg; ++s) p[s * elems] = run;
   }
   if (s1) s1[bh * elems + e] = run;

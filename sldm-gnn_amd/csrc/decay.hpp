@@ -236,12 +236,13 @@ __device__ __forceinline__ void zero_tail(const Args& a, const Role& R, const Sp
   }
 }
 
-// An infinity or NaN in a token's v would reach the outputs of the tokens in front of
-// it in the same chunk (as 0 times itself, in the masked half of P V), and in k
-// likewise.  It leaves a mark in the state that lasts to the end of the walk; a wave
-// that finds one there writes its columns' outputs anew by the recurrence itself,
-// token by token, where a token cannot reach what lies before it.  SPREAD: lanes
-// col + SPREAD, .. of the wave hold the other rows of a column.
+// A chunk's products mix its tokens, and a state's parts: an infinity or NaN in a
+// token's v would reach the outputs of the tokens in front of it in the same chunk (as
+// 0 times itself, in the masked half of P V), in k likewise, and where operands go in
+// as sums of terms an infinity would leave the state a NaN (as the difference of two).
+// It leaves a mark in the state that lasts to the end of the walk; a wave that finds
+// one there writes its columns' outputs and state anew by the recurrence itself, token
+// by token.  SPREAD: lanes col + SPREAD, .. of the wave hold the other rows of a column.
 template <int N>
 __device__ __forceinline__ bool finite(const float (&v)[N]) {
   float z = 0.f;
@@ -257,7 +258,7 @@ __device__ __forceinline__ int lane_again() {
 }
 __device__ __forceinline__ float widen(float v) { return v; }
 __device__ __forceinline__ float widen(uint16_t v) { return sldm::bf16_to_f32(v); }
-template <typename T, int N, int SPREAD, typename RowOf>
+template <typename T, int N, int SPREAD, bool OUT, typename RowOf>
 __device__ __forceinline__ void walk_tokens(const Args& a, int order, int which, int col, RowOf row_of) {
   asm volatile("" : "+s"(order));                // the role is read anew, not kept over the walk before
   const int id = a.by_roles.split(order);
@@ -267,7 +268,7 @@ __device__ __forceinline__ void walk_tokens(const Args& a, int order, int which,
 #pragma unroll
   for (int i = 0; i < N; ++i) S[i] = 0.f;
   if (R.s0) load_state(R, R.s0 + s.bh * R.s0_bh + s.seg * R.s0_seg, col, false, row_of, S);
-  const T* q = head_of<T>(a, R.q, s.b, s.hd);
+  const T* q = OUT ? head_of<T>(a, R.q, s.b, s.hd) : nullptr;
   const T* k = head_of<T>(a, R.k, s.b, s.hd);
   const T* v = head_of<T>(a, R.v, s.b, s.hd);
   const float g = exp2f(s.ld2), before = R.delta ? 1.f : g, after = R.delta ? g : 1.f;
@@ -283,11 +284,12 @@ __device__ __forceinline__ void walk_tokens(const Args& a, int order, int which,
       const int r = row_of(i);
       if (r < R.kd) {
         S[i] = S[i] * before + widen(k[t * R.k.st + r]) * vv;
-        o += widen(q[t * R.q.st + r]) * S[i];
+        if (OUT) o += widen(q[t * R.q.st + r]) * S[i];
         S[i] *= after;
       }
       if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
+    if (!OUT) continue;
 #pragma unroll
     for (int d = SPREAD; d < 64; d <<= 1) o += __shfl_xor(o, d);
     o *= R.read_scale;
@@ -297,6 +299,7 @@ __device__ __forceinline__ void walk_tokens(const Args& a, int order, int which,
       else reinterpret_cast<uint16_t*>(R.o)[at] = sldm::f32_to_bf16(o);
     }
   }
+  if (R.s1) store_state(R, R.s1 + s.bh * R.s1_bh + s.seg * R.s1_seg, col, false, row_of, S);
 }
 
 // Rows of a chunk within 32-bit byte offsets of each other.

@@ -330,7 +330,19 @@ __global__ __launch_bounds__(64 * NW, waves_for(tile_bytes<KT, NW, OUT>(), KT, N
     gn = gn_full;
   }
   if (OUT && nch > 0) put(nch - 1);
-  if (R.s1) {
+  bool clean = true;
+#pragma unroll
+  for (int t = 0; t < KT; ++t) {
+    float x[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = S[t][r];
+    clean = clean && finite(x);
+  }
+  if (!__all(clean)) {
+    const int l = lane_again();
+    walk_tokens<uint16_t, 16 * KT, 32, OUT>(a, order, 0, 32 * wave + perm16(l & 31),
+                                            [&](int i) { return 16 * (i >> 3) + 8 * (l >> 5) + (i & 7); });
+  } else if (R.s1) {
     float* s1 = R.s1 + sp.bh * R.s1_bh + sp.seg * R.s1_seg;
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
@@ -338,21 +350,6 @@ __global__ __launch_bounds__(64 * NW, waves_for(tile_bytes<KT, NW, OUT>(), KT, N
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[r] = S[t][r];
       store_state(R, s1, vc, whole, [&](int r) { return 32 * t + 16 * (r >> 3) + 8 * h + (r & 7); }, x);
-    }
-  }
-  if constexpr (OUT) {
-    bool clean = true;
-#pragma unroll
-    for (int t = 0; t < KT; ++t) {
-      float x[16];
-#pragma unroll
-      for (int r = 0; r < 16; ++r) x[r] = S[t][r];
-      clean = clean && finite(x);
-    }
-    if (!__all(clean)) {
-      const int l = lane_again();
-      walk_tokens<uint16_t, 16 * KT, 32>(a, order, 0, 32 * wave + perm16(l & 31),
-                                         [&](int i) { return 16 * (i >> 3) + 8 * (l >> 5) + (i & 7); });
     }
   }
   if constexpr (OUT) zero_tail<NTH, FAST>(a, R, sp, R.o_f32 ? 4 : 2);

@@ -234,7 +234,21 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_f32_kernel(Arg
     }
   }
   if (OUT && nt > 0) put(nt - 1);
-  if (R.s1) {
+  bool clean = true;
+#pragma unroll
+  for (int t = 0; t < KT; ++t)
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const float x[4] = {S[t][v][0], S[t][v][1], S[t][v][2], S[t][v][3]};
+      clean = clean && finite(x);
+    }
+  if (!__all(clean)) {
+    const int l = lane_again();
+#pragma unroll 1
+    for (int v = 0; v < NV; ++v)
+      walk_tokens<float, 4 * KT, 16, OUT>(a, order, which, v0 + 16 * v + (l & 15),
+                                          [&](int i) { return 16 * (i >> 2) + 4 * (l >> 4) + (i & 3); });
+  } else if (R.s1) {
     float* s1 = R.s1 + sp.bh * R.s1_bh + sp.seg * R.s1_seg;
 #pragma unroll
     for (int t = 0; t < KT; ++t)
@@ -243,23 +257,6 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_f32_kernel(Arg
         const float x[4] = {S[t][v][0], S[t][v][1], S[t][v][2], S[t][v][3]};
         store_state(R, s1, v0 + 16 * v + m, whole, [&](int r) { return 16 * t + 4 * h + r; }, x);
       }
-  }
-  if constexpr (OUT) {
-    bool clean = true;
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        const float x[4] = {S[t][v][0], S[t][v][1], S[t][v][2], S[t][v][3]};
-        clean = clean && finite(x);
-      }
-    if (!__all(clean)) {
-      const int l = lane_again();
-#pragma unroll 1
-      for (int v = 0; v < NV; ++v)
-        walk_tokens<float, 4 * KT, 16>(a, order, which, v0 + 16 * v + (l & 15),
-                                       [&](int i) { return 16 * (i >> 2) + 4 * (l >> 4) + (i & 3); });
-    }
   }
   if constexpr (OUT) zero_tail<PAIR ? 64 : NTH, FAST>(a, R, sp, 4);
 }
