@@ -236,19 +236,26 @@ __device__ __forceinline__ void zero_tail(const Args& a, const Role& R, const Sp
   }
 }
 
-// A chunk's products mix its tokens, and a state's parts: an infinity or NaN in a
+// A chunk's products mix its tokens, and a state's parts.  An infinity or NaN in a
 // token's v would reach the outputs of the tokens in front of it in the same chunk (as
-// 0 times itself, in the masked half of P V), in k likewise, and where operands go in
-// as sums of terms an infinity would leave the state a NaN (as the difference of two).
-// It leaves a mark in the state that lasts to the end of the walk; a wave that finds
-// one there writes its columns' outputs and state anew by the recurrence itself, token
-// by token.  SPREAD: lanes col + SPREAD, .. of the wave hold the other rows of a column.
-template <int N>
-__device__ __forceinline__ bool finite(const float (&v)[N]) {
-  float z = 0.f;
+// 0 times itself, in the masked half of P V), in k likewise; an infinity in q would
+// meet those zeros too, where operands go in as sums of terms one would become a NaN
+// (as the difference of two), and q k may leave fp32's range where q S does not.  All
+// of that leaves a mark in an output, or in the state, where it lasts to the end of
+// the walk; a wave that has seen one writes its columns' outputs and state anew by the
+// recurrence itself, token by token.  SPREAD: lanes col + SPREAD, .. of the wave hold
+// the other rows of a column.
+// seen: 0 while all are finite (and their sum is), NaN from then on.  N: a power of two.
+template <int N, typename V>
+__device__ __forceinline__ void mark(float& seen, const V& v) {
+  float x[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) z = __builtin_fmaf(v[i], 0.f, z);
-  return z == 0.f;
+  for (int i = 0; i < N; ++i) x[i] = v[i];
+#pragma unroll
+  for (int n = N / 2; n; n /= 2)
+#pragma unroll
+    for (int i = 0; i < n; ++i) x[i] += x[i + n];
+  seen = __builtin_fmaf(x[0], 0.f, seen);
 }
 // the lane's number, not kept in a register from the kernel's start
 __device__ __forceinline__ int lane_again() {

@@ -216,6 +216,7 @@ __global__ __launch_bounds__(64 * NW, waves_for(tile_bytes<KT, NW, OUT>(), KT, N
   const float* pd = dtab + 9 + m - 8 * h;                       // + 23 - (16 s + e): entry 32 + m - j
   const float* pw = wtab + 8 * h;
   f16v O;
+  float seen = 0.f;                                             // what mark() has found
   // chunk c's outputs: lane = token m, registers 8 s + e = columns 16 s + 8 h + e
   const int o_bytes = R.o_f32 ? 4 : 2;
   char* o_at = OUT ? reinterpret_cast<char*>(R.o) + (sp.b * R.o_sb + (int64_t)(sp.base + sign * (m - pad)) * R.o_st +
@@ -324,21 +325,16 @@ __global__ __launch_bounds__(64 * NW, waves_for(tile_bytes<KT, NW, OUT>(), KT, N
         O = mfma(vf[s], as_bf8(lo), O);
         O = mfma(vf[s], as_bf8(hi), O);
       }
+      mark<16>(seen, O);
     }
     update<KT>(S, vf, lk, ck, pw, gn);
     rd = rd_full;
     gn = gn_full;
   }
   if (OUT && nch > 0) put(nch - 1);
-  bool clean = true;
 #pragma unroll
-  for (int t = 0; t < KT; ++t) {
-    float x[16];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) x[r] = S[t][r];
-    clean = clean && finite(x);
-  }
-  if (!__all(clean)) {
+  for (int t = 0; t < KT; ++t) mark<16>(seen, S[t]);
+  if (!__all(seen == 0.f)) {
     const int l = lane_again();
     walk_tokens<uint16_t, 16 * KT, 32, OUT>(a, order, 0, 32 * wave + perm16(l & 31),
                                             [&](int i) { return 16 * (i >> 3) + 8 * (l >> 5) + (i & 7); });

@@ -121,6 +121,7 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_f32_kernel(Arg
   int row_x = (h ^ 4 * which ^ Swizzle<RBK>::of(m)) << 4, kcol_x = (m >> 2 ^ 4 * which ^ Swizzle<RBK>::of(4 * h)) << 4;
   const int vcol_x = (m >> 2 ^ Swizzle<RBV>::of(4 * h)) << 4;
   f4v O[SUB][NV];
+  float seen = 0.f;                                  // what mark() has found
   float* o_at = OUT ? reinterpret_cast<float*>(R.o) + sp.b * R.o_sb + (int64_t)(sp.base + sign * (m - pad)) * R.o_st +
                           sp.hd * R.o_sh + v0 + 4 * h
                     : nullptr;
@@ -212,6 +213,8 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_f32_kernel(Arg
         for (int r = 0; r < 4; ++r)
 #pragma unroll
           for (int v = 0; v < NV; ++v) O[s][v] = mfma(vv[v][r], P[r] * d[r], O[s][v]);
+#pragma unroll
+        for (int v = 0; v < NV; ++v) mark<4>(seen, O[s][v]);
       }
       const float gn = padc ? powg(ld2, C - padc) : gn_full;
       f4v kn = kcol(0);
@@ -234,15 +237,11 @@ __global__ __launch_bounds__(64 * NW, KT <= 2 ? 4 : 3) void decay_f32_kernel(Arg
     }
   }
   if (OUT && nt > 0) put(nt - 1);
-  bool clean = true;
 #pragma unroll
   for (int t = 0; t < KT; ++t)
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const float x[4] = {S[t][v][0], S[t][v][1], S[t][v][2], S[t][v][3]};
-      clean = clean && finite(x);
-    }
-  if (!__all(clean)) {
+    for (int v = 0; v < NV; ++v) mark<4>(seen, S[t][v]);
+  if (!__all(seen == 0.f)) {
     const int l = lane_again();
 #pragma unroll 1
     for (int v = 0; v < NV; ++v)

@@ -12,7 +12,7 @@ import pytest
 import torch
 
 from oracle import sequence_ref as ref
-from test_gpu_sequence import DEV, DTYPES, U, _decays, _gen, _randn, _within
+from test_gpu_sequence import DEV, U, _decays, _gen, _randn, _within
 
 pytestmark = pytest.mark.gpu
 TWO_TERMS = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -16}
@@ -43,12 +43,14 @@ def _both(q, k, v, ld, state, lengths, do, dend):
     return _oracle(*args), _oracle(*mags)
 
 
-def _finite_within(got, want, mag, dtype, T):
-    for name, a, w, m in zip(NAMES, got, want, mag):
+def _finite_within(got, want, mag, dtype, T, lost=None):
+    """lost: what else each may be off by (None: nothing)."""
+    for n, (name, a, w, m) in enumerate(zip(NAMES, got, want, mag)):
         fp32 = name in ("state", "dstate")
         u, two = (U[torch.float32], 0.0) if fp32 else (U[dtype], TWO_TERMS[dtype])
         fine = w.isfinite()
-        _within(a[fine], w[fine], _bound(u, two, T, w, m)[fine], name)
+        bound = _bound(u, two, T, w, m) + (0.0 if lost is None else lost[n])
+        _within(a[fine], w[fine], bound[fine], name)
 
 
 # B, T, H, Hk, Dk, Dv: one chunk and some, whole walks, a cut axis (shared heads, wide heads), rows element by element
