@@ -69,6 +69,14 @@ void once(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, ": the backward pass cannot be differentiated (create_graph=True)");
 }
 
+// Neither do forward-mode ones.  The kernels fill their outputs through pointers, so
+// that a tangent would be dropped, and read as zero, where no input requires grad.
+void no_tangents(const char* what, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), what,
+                " has no forward-mode derivative; detach the tangents (torch.autograd.forward_ad.unpack_dual)");
+}
+
 // --------------------------------------------------------------- layer norm --
 struct Rows {
   Tensor t;
@@ -154,6 +162,7 @@ Tensor layer_norm(const Tensor& x, const optional<Tensor>& weight, const optiona
                        "layer_norm: weight and bias are float32 or of the input's dtype, got ", t->scalar_type());
     }
   TORCH_CHECK_VALUE(eps >= 0, "layer_norm: eps must not be negative");
+  no_tangents("layer_norm", {&x, &w, &b});
   require_gpu("layer_norm", x, {&w, &b});
   if (at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b))) return NormFn::apply(x, weight, bias, eps);
   return norm_fwd(x, w, b, eps, nullptr);
@@ -270,6 +279,7 @@ std::tuple<Tensor, Tensor> rotary_axes(const Tensor& q, const optional<Tensor>& 
   const bool grad = at::GradMode::is_enabled();
   TORCH_CHECK(!(grad && (wants(positions) || wants(inv_freq))),
               "rotary_axes: positions and inv_freq have no gradient; detach them");
+  no_tangents("rotary_axes", {&q, &k, &positions, &inv_freq});
   require_gpu("rotary_axes", q, {&k, &positions, &inv_freq});
   if (grad && (wants(q) || wants(k))) {
     auto r = RotaryFn::apply(q, k_in, positions, inv_freq, sections.vec(), interleaved);
@@ -408,6 +418,7 @@ std::tuple<Tensor, Tensor> decay_attention(const Tensor& q, const Tensor& k, con
     TORCH_CHECK_VALUE(lengths.dim() == 1 && lengths.size(0) == d.B, "decay_attention: lengths are [", d.B, "], got ",
                       lengths.sizes());
   }
+  no_tangents(what, {&q, &k, &v, &log_decay, &state});
   require_gpu(what, q, {&k, &v, &log_decay, &state, &lengths});
   const double scale = scale_in.has_value() ? *scale_in : 1.0 / std::sqrt((double)d.dk);
   optional<Tensor> lens = lengths_in;
@@ -431,6 +442,7 @@ Tensor decay_attention_step(const Tensor& q_in, const Tensor& k_in, const Tensor
   TORCH_CHECK_VALUE(state.is_contiguous(), what, ": the state is moved on in place and has to be contiguous");
   TORCH_CHECK(!(at::GradMode::is_enabled() && (wants(q_in) || wants(k_in) || wants(v_in) || wants(state))), what,
               " moves the state on in place and has no gradient; use decay_attention, or torch.no_grad()");
+  no_tangents(what, {&q_in, &k_in, &v_in, &log_decay, &state});
   require_gpu(what, q_in, {&k_in, &v_in, &log_decay, &state});
   DeviceGuard guard(q_in.device());
   const Tensor q = cols(q_in), k = cols(k_in), v = cols(v_in), g = log_decay.contiguous();

@@ -13,7 +13,7 @@ in and comes out, so live data can go on frame by frame:
 
 :class:`LayerNorm` and :class:`DecayEncoder` are the modules over them.  All
 run on ROCm tensors in float32 or bfloat16 on the current stream; CPU tensors
-raise (no fallback).  Kernels: csrc/norm.hip, rotary.hip, decay.hip; operators
+raise (no fallback), and so do second and forward-mode derivatives.  Kernels: csrc/norm.hip, rotary.hip, decay.hip; operators
 with their autograd: csrc/sequence_ops.cpp (``torch.ops.sldm``).
 """
 from __future__ import annotations

@@ -1,0 +1,31 @@
+"""Calls of the sequence operators that have no answer and are refused; no kernel runs (CPU tensors)."""
+from __future__ import annotations
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+import sldm_sage as sage
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A tangent would be dropped without a word, and read as a derivative of zero."""
+    x, w = torch.randn(3, 8), torch.ones(8)
+    q, pos, f = torch.zeros(2, 5, 2, 16), torch.zeros(2, 5, 1), sage.rotary_frequencies((8,))
+    ld, state = torch.zeros(2), torch.zeros(2, 2, 16, 16)
+    calls = [(sage.layer_norm, (x, w, w)), (sage.rotary_axes, (q, q, pos, f, (8,))),
+             (lambda q, k, v, ld, s: sage.decay_attention(q, k, v, ld, state=s), (q, q, q, ld, state)),
+             (sage.decay_attention_step, (q[:, 0], q[:, 0], q[:, 0], ld, state))]
+    for call, args in calls:
+        for i, a in enumerate(args):
+            if not isinstance(a, torch.Tensor):
+                continue
+            for leaf in (False, True):
+                with forward_ad.dual_level():
+                    dual = forward_ad.make_dual(a.detach().clone(), torch.ones_like(a))
+                    if leaf:
+                        dual.requires_grad_(True)
+                    with pytest.raises(RuntimeError, match="forward-mode|no gradient"), torch.set_grad_enabled(leaf):
+                        call(*args[:i], dual, *args[i + 1:])
+            with forward_ad.dual_level(), pytest.raises(RuntimeError, match="no CPU fallback"):
+                call(*args)                            # no tangent: on to the next check
