@@ -182,12 +182,24 @@ class DecayEncoder(nn.Module):
     def _out(self, h, o):
         return h + self.proj(self.head_norm(o).flatten(-2))
 
+    def _state(self, state, n: int, whole: bool):
+        """(S, seen) of ``n`` sequences; ``whole``: neither may be None."""
+        want = [(n, self.num_heads, self.head_dim, self.head_dim), (n,)]
+        ok = isinstance(state, (tuple, list)) and len(state) == 2 and all(
+            t is None and not whole or isinstance(t, torch.Tensor) and tuple(t.shape) == size
+            for t, size in zip(state, want))
+        if not ok:
+            got = tuple(tuple(t.shape) if isinstance(t, torch.Tensor) else t for t in state) \
+                if isinstance(state, (tuple, list)) else type(state).__name__
+            raise ValueError(f"DecayEncoder: the state is (S {list(want[0])}, tokens seen [{n}]), got {got}")
+        return state
+
     def forward(self, x: torch.Tensor, state=None, positions: torch.Tensor | None = None,
                 lengths: torch.Tensor | None = None):
         if x.dim() != 3 or x.size(-1) != self.input_size:
             raise ValueError(f"DecayEncoder: expected [N, T, {self.input_size}], got {tuple(x.shape)}")
         N, T = x.shape[:2]
-        S, seen = (None, None) if state is None else state
+        S, seen = (None, None) if state is None else self._state(state, N, whole=False)
         if seen is None:
             seen = torch.zeros(N, dtype=torch.int64, device=x.device)
         if positions is None:
@@ -201,7 +213,9 @@ class DecayEncoder(nn.Module):
     def step(self, x: torch.Tensor, state, positions: torch.Tensor | None = None):
         """One frame ``x [N, input_size]``; ``state`` (of an earlier call, or :meth:`init_state`) is moved
         on in place.  Returns ``out [N, hidden_size]``."""
-        S, seen = state
+        if x.dim() != 2 or x.size(-1) != self.input_size:
+            raise ValueError(f"DecayEncoder.step: expected [N, {self.input_size}], got {tuple(x.shape)}")
+        S, seen = self._state(state, x.size(0), whole=True)
         if positions is None:
             positions = seen[:, None].expand(-1, len(self.sections))
         h, q, k, v = self._qkv(x, positions)

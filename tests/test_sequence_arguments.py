@@ -29,3 +29,27 @@ def test_forward_mode_derivatives_are_refused():
                         call(*args[:i], dual, *args[i + 1:])
             with forward_ad.dual_level(), pytest.raises(RuntimeError, match="no CPU fallback"):
                 call(*args)                            # no tangent: on to the next check
+
+
+def test_encoder_state_and_frame_are_checked():
+    enc = sage.DecayEncoder(6, 96, num_heads=6)
+    S, seen = enc.init_state(3)
+    frame, frames = torch.zeros(3, 6), torch.zeros(3, 4, 6)
+    for x in (torch.zeros(3, 7), torch.zeros(6), frames):
+        with pytest.raises(ValueError, match=r"expected \[N, 6\]"):
+            enc.step(x, (S, seen))
+    for state in (S, None, (S,), (S, seen, seen), (S[:2], seen), (S, seen[:2]), (S, seen[:, None]), (S[..., :8], seen),
+                  (S, 3), (seen, S)):
+        with pytest.raises(ValueError, match="state is"):
+            enc.step(frame, state)
+        if state is not None:
+            with pytest.raises(ValueError, match="state is"):
+                enc(frames, state)
+    for state in ((None, seen), (S, None)):
+        with pytest.raises(ValueError, match="state is"):
+            enc.step(frame, state)
+    assert not seen.any() and not S.any()
+    for call in (lambda: enc.step(frame, (S, seen)), lambda: enc(frames, (S, seen)), lambda: enc(frames, (S, None)),
+                 lambda: enc(frames, (None, seen))):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            call()
