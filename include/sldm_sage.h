@@ -446,7 +446,7 @@ int sldm_rotary_axes(int dtype, const void* q, const int64_t* ld_q, int64_t head
  * [B, H, dk, dv] fp32 contiguous: the state before the first token and behind
  * the last.  lengths (device [B], int32 or int64, nullable: T): tokens from
  * lengths[b] on (clamped to [0, T]) are padding: not read into the state, their
- * outputs are zeros.  out [B, T, H, dv] contiguous.  1 <= dk, dv <= 128.
+ * outputs are zeros.  out [B, T, H, dv] contiguous.  1 <= dk, dv <= 128, B H < 2^22.
  * log_decay [H] fp32, <= 0 (-inf: nothing is kept).
  * A long axis with few (batch, head) pairs is cut into segments; `states`
  * (sldm_decay_attention_states_bytes bytes; 0: may be NULL) then takes the

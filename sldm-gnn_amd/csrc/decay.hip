@@ -18,11 +18,15 @@ constexpr int kChunk = 32;   // tokens of a segment are a multiple of this: no p
 // leaves the chip short of waves; then the axis is cut, at the price of a pass
 // over k and v for the pieces' states, which are read and written too.  Fewer
 // than four pieces do not pay for that pass (bf16, 64 heads of 64, 1024 frames:
-// 59 us whole, 54 us in two, 40 in four; 128 heads, 512 frames: 34, 40, 37), nor
-// do short ones, nor fewer than five in fp32 (1024 heads of 16, 2048 frames: 111 us
-// whole, 168 us in four).  Waves aimed at, of 8 / 12 / 16 a CU: bf16 (8 heads of 128,
-// 32768 frames, training) 365 / 397 / 438 us, with 8 for the forward alone 350 /
-// 334 / - us; fp32 (8 heads of 48 and 80, 1237 frames, training) 264 / 221 / 211 us.
+// 51 us whole, 48 us in two, 33 in four; 128 heads, 512 frames: 29, 33, 32), nor
+// do short ones, nor in fp32 so few waves missing that fewer than five would make them
+// up (1024 heads of 16, 2048 frames: 115 us whole, 194 us in four).  Where only the
+// length allows no more than four, those pay in fp32 for few heads (544 frames, 8 heads
+// of 64: 66 us whole, 41 in four, training 130 and 83) and not quite for many (192
+// heads: 66 and 81, 178 and 192).  Waves aimed at, of 8 / 12 / 16 a CU: bf16 (8 heads
+// of 128, 32768 frames, training) 392 / 393 / 430 us, with 8 for the forward and 12 for
+// the backward 380; fp32 (5 x 1237 frames, 8 over 2 heads of 48 and 80, training) 305 /
+// 159 / 158 us.
 struct Plan {
   int64_t seg_len;
   int nseg;
@@ -126,8 +130,9 @@ __global__ __launch_bounds__(256) void sum_heads_kernel(SumArgs a) {
 // One token: S <- g S + k v^T and o = scale q S, the state read and written
 // once (its 8 Dk Dv bytes are all that counts).  A workgroup owns one (batch,
 // head); lanes hold V neighbouring value columns, the row groups' partial sums
-// of o meet in LDS.  Measured: 512 x 16 states of 64 x 64 56 us (4.9 TB/s), 240 of
-// 16 x 16 3.9 us.
+// of o meet in LDS.  Measured: 512 x 16 states of 64 x 64 56 us a pass on states that
+// change (4.9 TB/s), 43 us on the same ones (6.4 TB/s, partly from the Infinity Cache);
+// 240 of 16 x 16 4.5 us.
 struct StepArgs {
   const void *q, *k, *v;
   int64_t q_sb, q_sh, k_sb, k_sh, v_sb, v_sh;

@@ -9,6 +9,9 @@
 //   S' <- g^C S + K^T diag(g^{C-1-j}) V
 // Every exponent is >= 0, so no decay, however strong, overflows.
 //
+// A product q_i k_j inside a chunk that is smaller than its type's smallest number is
+// lost (bf16 and fp32: steps of 2^-133 and 2^-149), whatever v_j it meets.
+//
 // The gradients are the same recurrence with other operands
 //   dq_t = scale S_t do_t                              q,k,v := do, v, k   (S^T)
 //   G_t  = scale q_t do_t^T + g G_{t+1}                time reversed
@@ -244,7 +247,9 @@ __device__ __forceinline__ void zero_tail(const Args& a, const Role& R, const Sp
 // of that leaves a mark in an output, or in the state, where it lasts to the end of
 // the walk; a wave that has seen one writes its columns' outputs and state anew by the
 // recurrence itself, token by token.  SPREAD: lanes col + SPREAD, .. of the wave hold
-// the other rows of a column.
+// the other rows of a column.  Looking costs 1 % (57600 heads of 16, 100 frames, training: 907
+// -> 918 us); a walk about 5 us a token and wave (1024 heads of 64, 2048 frames, a NaN in
+// each: 9.9 ms).
 // seen: 0 while all are finite (and their sum is), NaN from then on.  N: a power of two.
 template <int N, typename V>
 __device__ __forceinline__ void mark(float& seen, const V& v) {

@@ -12,11 +12,12 @@
 // spread over the banks.  Chunks of 64 (half as many state conversions) were
 // slower: their tiles and accumulators leave two waves a SIMD and spill.
 //
-// Measured (MI355X; copies 4.76 TB/s).  1024 heads, 2048 frames: 64-wide 228 us
-// (4.7 TB/s), 128-wide 503 us (4.3 TB/s), bound by memory; 16-wide 80 us (3.4
-// TB/s) and few long heads by the chain of a chunk (about 1 us from its first read
-// to its state).  8 heads of 128, 32768 frames: forward 41 us for the segments'
-// states, 14 for the scan, 59 for the outputs, backward 41, 14 and 160.
+// Measured (MI355X; copies reach 4.6 to 6.3 TB/s).  1024 sequences of one head, 2048
+// frames: 64-wide 226 us (4.7 TB/s), bound by memory; 128-wide 552 us (3.9 TB/s) by
+// VALU and MFMA issue; 16-wide 84 us (3.2 TB/s) and few long heads by the chain of a
+// chunk (about 1 us from its first read to its state).  8 heads of 128, 32768 frames:
+// forward 43 us for the segments' states, 15 for the scan, 78 to 85 for the outputs,
+// backward 43, 15 and 213 to 222 (MFMA 45 %, VALU 64 % of the time busy).
 //
 // Roundings.  The state is held in fp32 accumulators.  What the matrix instructions
 // take from fp32 goes in as sums of bf16 terms: the state that is read, and P = Q K^T
@@ -24,7 +25,9 @@
 // at most 2^-16 of themselves, far below what rounding the output to bf16 costs), and
 // V g^{n-1-j}, which enters the state, as hi + mid + lo (all 24).  One term for the
 // state or for P would be as large an error as the output's own rounding (relative
-// error 0.0024 instead of 0.0017), and more where the products cancel.
+// error 0.0024 instead of 0.0017), and more where the products cancel.  What the second
+// terms cost: 32768 frames, 8 heads of 128, training 316 -> 391 us with the third term
+// into the state (345 with two), 64-wide heads nothing that shows.
 #pragma once
 
 #include "decay.hpp"

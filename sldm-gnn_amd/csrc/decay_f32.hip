@@ -11,11 +11,12 @@
 // cost C (Dk + Dv) a token against 2 Dk Dv between chunks, and a 16-wide head
 // wastes no part of a tile.
 //
-// Measured (MI355X; copies 4.76 TB/s, an fp32 matrix product 153 TFLOP/s).  1024
-// heads, 2048 frames: 16-wide 112 us (4.8 TB/s) and 64-wide 490 us (4.4 TB/s),
-// bound by memory; 128-wide 1.49 ms, 121 TFLOP/s of issued products, bound by
-// them.  57600 heads of 16, 100 frames: forward 290 us (5.1 TB/s), backward 610 us
-// (4.2 TB/s of q, k, v, do, dq, dk, dv once each).
+// Measured (MI355X; copies reach 4.6 to 6.3 TB/s, an fp32 matrix product 153 TFLOP/s).
+// 1024 sequences of one head, 2048 frames: 16-wide 109 us (4.9 TB/s) and 64-wide 471 us
+// (4.6 TB/s), bound by memory; 128-wide 1.47 ms, 123 TFLOP/s of issued products, bound
+// by them.  57600 heads of 16, 100 frames: forward 270 us (5.7 TB/s), backward 630 to 670
+// us (4.0 TB/s of q, k, v, do, dq, dk, dv once each, which is all that moves); in the
+// first ten passes after a pause 315 and up to 870 us.
 #include "decay.hpp"
 
 namespace sldm_decay {

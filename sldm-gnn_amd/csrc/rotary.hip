@@ -10,7 +10,7 @@
 // (positions of 10^6 times a frequency of 1 leave fp32 an error of 0.06), and
 // only then rounded for the fp32 sine and cosine.
 //
-// Measured (MI355X, copies at 4.76 TB/s): 960 000 tokens x 12 heads of 16, fp32,
+// Measured (MI355X, copies at 4.6 to 6.3 TB/s): 960 000 tokens x 12 heads of 16, fp32,
 // 291 us (5.1 TB/s); 32768 tokens x 20 heads of 128, bf16, 67 us (5.0 TB/s); 300
 // tokens x 12 heads of 16, bf16, 4.7 us.
 #include <algorithm>

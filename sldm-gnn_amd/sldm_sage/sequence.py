@@ -80,7 +80,8 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
         S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T        out_t = scale q_t S_t
 
     ``q`` ``[B, T, H, Dk]``, ``k`` ``[B, T, Hk, Dk]``, ``v`` ``[B, T, Hk, Dv]`` (float32 or
-    bfloat16; ``Hk`` divides ``H``, head h reads key head ``h // (H // Hk)``; sizes 1 to 128);
+    bfloat16; ``Hk`` divides ``H``, head h reads key head ``h // (H // Hk)``; sizes 1 to 128;
+    ``B * H`` below 2^22);
     ``log_decay`` float32 ``[H]``, not above 0; ``scale`` defaults to ``Dk ** -0.5``; ``state``
     float32 ``[B, H, Dk, Dv]`` is the state before the first token (None: zeros) and the returned
     one that behind the last.  ``lengths`` (int32 or int64 ``[B]``, clamped to ``[0, T]``): later
